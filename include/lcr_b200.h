@@ -413,6 +413,133 @@ LCR_API int lcr_batch_step_launches(const lcr_batch* batch, int n);
  * positions) between CUDA events on the batch stream: ms in total. */
 LCR_API int lcr_batch_time_steps(lcr_batch* batch, int steps, float* ms);
 
+/* ------------------------------------------------------------------------- */
+/* Ragged steps over a paged cache -- no counterpart in the reference, whose   */
+/* Model takes one sequence at a time. In one step every request brings its    */
+/* own number of new tokens: one, a few drafted tokens, a chunk of its prompt. */
+/* The page tables live on the device; per step: lcr_plan_step, then per layer */
+/* the projections with lcr_qk_norm_rope_kv and lcr_chunk_attention, then      */
+/* lcr_token_probs and lcr_verify_drafts on the rows of logits.                */
+/*                                                                             */
+/* All arrays are device memory, calls are asynchronous on `stream` and        */
+/* allocate nothing, so they may be captured in a graph. A step's rows are     */
+/* packed: request b owns rows row_starts[b] .. row_starts[b + 1] - 1. The     */
+/* cache is an lcr_kv_view whose keys / values are pools of pool_pages pages:  */
+/* page p, KV head h, slot s at p * page_stride + h * head_stride + s *        */
+/* head_dim elements (64-bit offsets; the strides multiples of 8 elements);    */
+/* view->page_table is the requests' tables, [sequences][max_pages] physical   */
+/* pages. Any page_size from 1 up.                                             */
+/* ------------------------------------------------------------------------- */
+
+#define LCR_PLAN_MAX_SEQUENCES 8192
+
+/* Block tables, slot map and row map of a step, from the requests' lengths.
+ *
+ * Request b has cached[b] positions in the cache and brings new_tokens[b]
+ * more (0 = idle in this step; negative counts as 0). Its row of block_tables
+ * holds held[b] pages. With finished[b] != 0 (finished may be NULL) the slot
+ * is being turned over: its pages go back to the free stack first and it
+ * holds none; cached[b] and new_tokens[b] then describe the slot's next
+ * request (0, 0 for an empty slot).
+ *
+ * The free pages are a stack, free_pages[0 .. *free_count - 1], in a buffer of
+ * pool_pages entries. Pages given back are pushed in request order, then each
+ * request takes what it lacks for cached + new positions from the top, in
+ * request order. When the stack runs out, the requests that still lack pages
+ * are refused: they take none (nor does a request that needs more than
+ * max_pages), their kv_lengths are 0 and their rows have no slots.
+ *
+ * Out: block_tables (in place), held_out and free_count_out (which may be
+ * held and free_count themselves), row_starts [sequences + 1], kv_lengths
+ * [sequences] (cached + new, 0 if refused), and for each row r < max_rows its
+ * positions[r], slots[r] = page * page_size + position % page_size (-1 if
+ * refused) and row_sequence[r] = b. Rows past max_rows are cut off.
+ * pool_pages * page_size must fit in 31 bits. */
+LCR_API int lcr_plan_step(int32_t* block_tables, int max_pages, const int32_t* held, int32_t* held_out,
+                          int32_t* free_pages, const int32_t* free_count, int32_t* free_count_out,
+                          int pool_pages, const int32_t* cached, const int32_t* new_tokens,
+                          const int32_t* finished, int sequences, int page_size, int max_rows,
+                          int32_t* row_starts, int32_t* kv_lengths, int32_t* positions, int32_t* slots,
+                          int32_t* row_sequence, lcr_stream_t stream);
+
+/* Per-head RMSNorm of q and k, rotary positions, and the cache write, in one
+ * pass over the projection's output. Row r of qkv holds num_heads query
+ * heads, then num_kv_heads key and value heads, of head_dim (64 or 128)
+ * elements. Each q and k head x becomes x * rsqrt(mean(x^2) + eps) * gain
+ * (q_gain / k_gain [head_dim] bf16; NULL = no norm), then is rotated
+ * (rotate-half, angle = positions[r] * inv_freq[i], i < head_dim / 2) -- all
+ * in fp32, rounded to bf16 once. q goes to q_out (row stride q_stride), k and
+ * v to slot slots[r] of the pools (page slots[r] / page_size); a row whose
+ * slot is outside the pool (-1) writes no K / V. Rows of one call must have
+ * distinct slots. q_out may be qkv itself (with q_stride = qkv_stride).
+ * Strides in elements, multiples of 8; buffers 16-byte aligned. */
+LCR_API int lcr_qk_norm_rope_kv(void* q_out, int64_t q_stride, const lcr_kv_view* view, int pool_pages,
+                                const void* qkv, int64_t qkv_stride, int rows, int num_heads,
+                                const void* q_gain, const void* k_gain, float eps, const float* inv_freq,
+                                const int32_t* positions, const int32_t* slots, lcr_stream_t stream);
+
+/* Attention of every request's new rows over its pages. Row i of the n rows
+ * of request b sits at position p = kv_lengths[b] - n + i and attends to the
+ * cached positions 0 .. p (its own and earlier new tokens' K / V are in the
+ * cache already): out = softmax(scale * q k) v, query head h on KV head
+ * h / (num_heads / num_kv_heads). A row with no position (p < 0, e.g. of a
+ * refused request) gives zeros. head_dim 64 or 128, any number of query heads
+ * per KV head up to 128. q and out: [rows][num_heads * head_dim] with row
+ * strides in elements (multiples of 8), 16-byte aligned, not overlapping.
+ * kv_lengths past max_pages * page_size are cut to it, and a table entry
+ * outside the pool reads as zeros, with status LCR_ERR_POOL. The keys and
+ * values of positions below kv_lengths must be finite; the rest of a page is
+ * never read.
+ *
+ * scratch: lcr_chunk_attention_scratch_bytes(num_heads, head_dim) bytes,
+ * 16-byte aligned, zeroed once before its first use; every call leaves it
+ * ready for the next. Calls that may overlap need scratch of their own. */
+LCR_API int lcr_chunk_attention(void* out, int64_t out_stride, const void* q, int64_t q_stride,
+                                const lcr_kv_view* view, int max_pages, int pool_pages,
+                                const int32_t* row_starts, const int32_t* kv_lengths, int sequences, int rows,
+                                int num_heads, float scale, void* scratch, size_t scratch_bytes,
+                                lcr_stream_t stream);
+LCR_API size_t lcr_chunk_attention_scratch_bytes(int num_heads, int head_dim);
+/* What the calls on this scratch have reported since the last query, which
+ * clears it: LCR_OK, LCR_ERR_POOL (a table entry outside the pool) or
+ * LCR_ERR_TIMEOUT. Waits for the stream. */
+LCR_API int lcr_chunk_attention_status(void* scratch, lcr_stream_t stream);
+
+/* Rows of fp32 logits to probabilities: probs = softmax(logits / t) with t =
+ * temperature[row_sequence[r]] (row_sequence NULL: temperature[r];
+ * temperature NULL: 1); t <= 0 puts everything on the largest logit (lowest
+ * id on ties). Logits of -inf get 0, and a row of nothing but -inf is all
+ * zeros. probs may be logits itself. Row strides in elements. */
+LCR_API int lcr_token_probs(float* probs, int64_t probs_stride, const float* logits, int64_t logits_stride,
+                            int rows, int vocab, const float* temperature, const int32_t* row_sequence,
+                            lcr_stream_t stream);
+
+/* Verification of drafted tokens by given random numbers, so that the tokens
+ * kept are distributed as the target's own samples.
+ *
+ * Request b's target distributions are rows target_starts[b] ..
+ * target_starts[b + 1] - 1 of target_probs (none: an idle request); the last
+ * k + 1 of them, k = draft_counts[b], follow its last kept token and its
+ * drafts drafts[b][0 .. k - 1]. draft_probs [sequences][max_drafts][vocab]
+ * holds what each draft was drawn from (NULL: each draft is certain, as from
+ * a table look-up). Probabilities count in units of 2^-38 (P = p * 2^38
+ * rounded to nearest even; below 0 and NaN as 0, above 1 as 1) and uniforms
+ * [sequences][max_drafts + 1] in [0, 1) in units of 2^-24 (rounded down), so
+ * the results are whole numbers' and do not depend on any order of summation:
+ *   draft j is kept while U_j * Q_j(d_j) < P_j(d_j) * 2^24;
+ *   at the first refusal j the next token is drawn from R = max(P_j - Q_j, 0)
+ *   (from P_j if that is 0 everywhere), after k kept drafts from R = P_k: the
+ *   lowest x whose running sum exceeds U * sum(R) / 2^24 (rounded down), U of
+ *   uniforms[b][max_drafts].
+ * tokens[b][0 .. max_drafts] = the kept drafts, the drawn token, then -1;
+ * accepted[b] = drafts kept. Idle requests, and a draw from nothing but
+ * zeros, give -1. A draft outside the vocabulary is refused. k is cut to
+ * max_drafts and to the request's rows. */
+LCR_API int lcr_verify_drafts(int32_t* tokens, int32_t* accepted, const float* target_probs,
+                              int64_t target_stride, const int32_t* target_starts, const int32_t* drafts,
+                              const int32_t* draft_counts, const float* draft_probs, const float* uniforms,
+                              int sequences, int max_drafts, int vocab, lcr_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

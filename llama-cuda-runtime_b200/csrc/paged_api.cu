@@ -1,0 +1,197 @@
+// C entry points of the ragged step over a paged cache (include/lcr_b200.h):
+// argument checks and launches.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "chunk_attn.cuh"
+#include "common.cuh"
+#include "lcr_b200.h"
+#include "qk_norm_rope.cuh"
+#include "step_plan.cuh"
+#include "token_probs.cuh"
+#include "verify_drafts.cuh"
+
+using namespace lcrb;
+
+namespace {
+
+cudaStream_t cs(lcr_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// What lcr_qk_norm_rope_kv and lcr_chunk_attention ask of a cache.
+int check_view(const char* what, const lcr_kv_view* v, int pool_pages) {
+  LCRB_REQUIRE(v && v->keys && v->values, LCR_ERR_INVALID, "%s: null cache", what);
+  LCRB_REQUIRE(v->page_size > 0 && v->num_kv_heads > 0 && pool_pages > 0, LCR_ERR_INVALID,
+               "%s: page size %d, %d KV heads, %d pool pages", what, v->page_size, v->num_kv_heads, pool_pages);
+  LCRB_REQUIRE(v->head_dim == 64 || v->head_dim == 128, LCR_ERR_SHAPE, "%s is compiled for head_dim 64 or 128, got %d",
+               what, v->head_dim);
+  LCRB_REQUIRE(v->page_stride > 0 && v->head_stride > 0 && v->page_stride % 8 == 0 && v->head_stride % 8 == 0 &&
+                   aligned16(v->keys) && aligned16(v->values),
+               LCR_ERR_SHAPE, "%s needs 16-byte aligned cache rows (strides %d, %d)", what, v->page_stride,
+               v->head_stride);
+  LCRB_REQUIRE(static_cast<long long>(pool_pages) * v->page_size <= INT32_MAX, LCR_ERR_SHAPE,
+               "%s: a pool of %d pages of %d positions passes 31 bits", what, pool_pages, v->page_size);
+  return LCR_OK;
+}
+
+}  // namespace
+
+extern "C" int lcr_plan_step(int32_t* block_tables, int max_pages, const int32_t* held, int32_t* held_out,
+                             int32_t* free_pages, const int32_t* free_count, int32_t* free_count_out, int pool_pages,
+                             const int32_t* cached, const int32_t* new_tokens, const int32_t* finished, int sequences,
+                             int page_size, int max_rows, int32_t* row_starts, int32_t* kv_lengths,
+                             int32_t* positions, int32_t* slots, int32_t* row_sequence, lcr_stream_t stream) {
+  LCRB_REQUIRE(sequences > 0 && max_pages > 0 && pool_pages > 0 && page_size > 0 && max_rows >= 0, LCR_ERR_INVALID,
+               "plan_step: %d requests, %d pages each, pool of %d pages of %d, %d rows", sequences, max_pages,
+               pool_pages, page_size, max_rows);
+  LCRB_REQUIRE(block_tables && held && held_out && free_pages && free_count && free_count_out && cached && new_tokens &&
+                   row_starts && kv_lengths && (max_rows == 0 || (positions && slots && row_sequence)),
+               LCR_ERR_INVALID, "plan_step: null pointer");
+  LCRB_REQUIRE(sequences <= LCR_PLAN_MAX_SEQUENCES, LCR_ERR_SHAPE, "plan_step: %d requests; at most %d", sequences,
+               LCR_PLAN_MAX_SEQUENCES);
+  LCRB_REQUIRE(static_cast<long long>(sequences) * max_pages <= INT32_MAX &&
+                   static_cast<long long>(pool_pages) * page_size <= INT32_MAX,
+               LCR_ERR_SHAPE, "plan_step: tables or pool pass 31 bits");
+  StepPlanArgs a = {block_tables, max_pages,  held,      held_out,   free_pages, free_count, free_count_out,
+                    pool_pages,   cached,     new_tokens, finished,   sequences,  page_size,  max_rows,
+                    row_starts,   kv_lengths, positions, slots,      row_sequence};
+  const size_t smem = sizeof(int32_t) * 4 * static_cast<size_t>(sequences);
+  LCRB_CUDA(cudaFuncSetAttribute(step_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  return launch_kernel(step_plan_kernel, dim3(1), dim3(kPlanThreads), smem, cs(stream), false, a);
+}
+
+extern "C" int lcr_qk_norm_rope_kv(void* q_out, int64_t q_stride, const lcr_kv_view* view, int pool_pages,
+                                   const void* qkv, int64_t qkv_stride, int rows, int num_heads, const void* q_gain,
+                                   const void* k_gain, float eps, const float* inv_freq, const int32_t* positions,
+                                   const int32_t* slots, lcr_stream_t stream) {
+  if (rows == 0) return LCR_OK;
+  LCRB_REQUIRE(q_out && qkv && inv_freq && positions && slots && rows > 0 && num_heads > 0 && eps >= 0.f,
+               LCR_ERR_INVALID, "qk_norm_rope_kv: null pointer or bad size");
+  LCRB_TRY(check_view("qk_norm_rope_kv", view, pool_pages));
+  const int64_t width = static_cast<int64_t>(num_heads + 2 * view->num_kv_heads) * view->head_dim;
+  LCRB_REQUIRE(qkv_stride >= width && q_stride >= static_cast<int64_t>(num_heads) * view->head_dim, LCR_ERR_INVALID,
+               "qk_norm_rope_kv: row strides %lld (of %lld elements) and %lld", static_cast<long long>(qkv_stride),
+               static_cast<long long>(width), static_cast<long long>(q_stride));
+  LCRB_REQUIRE(qkv_stride % 8 == 0 && q_stride % 8 == 0 && aligned16(qkv) && aligned16(q_out) && aligned16(q_gain) &&
+                   aligned16(k_gain),
+               LCR_ERR_SHAPE, "qk_norm_rope_kv needs 16-byte aligned rows and gains");
+  QkNormRopeArgs a = {};
+  a.q_out = static_cast<bf16*>(q_out);
+  a.q_stride = q_stride;
+  a.keys = static_cast<bf16*>(view->keys);
+  a.values = static_cast<bf16*>(view->values);
+  a.page_stride = view->page_stride;
+  a.head_stride = view->head_stride;
+  a.page_size = view->page_size;
+  a.pool_pages = pool_pages;
+  a.qkv = static_cast<const bf16*>(qkv);
+  a.qkv_stride = qkv_stride;
+  a.rows = rows;
+  a.heads = num_heads;
+  a.kv_heads = view->num_kv_heads;
+  a.q_gain = static_cast<const bf16*>(q_gain);
+  a.k_gain = static_cast<const bf16*>(k_gain);
+  a.eps = eps;
+  a.inv_freq = inv_freq;
+  a.positions = positions;
+  a.slots = slots;
+  auto kernel = view->head_dim == 64 ? qk_norm_rope_kernel<64> : qk_norm_rope_kernel<128>;
+  return launch_kernel(kernel, dim3(static_cast<unsigned>(rows)), dim3(kQkThreads), 0, cs(stream), false, a);
+}
+
+extern "C" size_t lcr_chunk_attention_scratch_bytes(int num_heads, int head_dim) {
+  (void)num_heads;
+  (void)head_dim;
+  return 256;
+}
+
+extern "C" int lcr_chunk_attention(void* out, int64_t out_stride, const void* q, int64_t q_stride,
+                                   const lcr_kv_view* view, int max_pages, int pool_pages, const int32_t* row_starts,
+                                   const int32_t* kv_lengths, int sequences, int rows, int num_heads, float scale,
+                                   void* scratch, size_t scratch_bytes, lcr_stream_t stream) {
+  if (rows == 0 || sequences == 0) return LCR_OK;
+  LCRB_REQUIRE(out && q && row_starts && kv_lengths && scratch && sequences > 0 && rows > 0 && num_heads > 0 &&
+                   max_pages > 0,
+               LCR_ERR_INVALID, "chunk_attention: null pointer or bad size");
+  LCRB_TRY(check_view("chunk_attention", view, pool_pages));
+  LCRB_REQUIRE(view->page_table != nullptr, LCR_ERR_INVALID, "chunk_attention: no page tables");
+  LCRB_REQUIRE(num_heads % view->num_kv_heads == 0 && num_heads / view->num_kv_heads <= 128, LCR_ERR_SHAPE,
+               "chunk_attention: %d query heads on %d KV heads", num_heads, view->num_kv_heads);
+  const int64_t width = static_cast<int64_t>(num_heads) * view->head_dim;
+  LCRB_REQUIRE(q_stride >= width && out_stride >= width, LCR_ERR_INVALID,
+               "chunk_attention: row strides %lld and %lld of %lld elements", static_cast<long long>(q_stride),
+               static_cast<long long>(out_stride), static_cast<long long>(width));
+  LCRB_REQUIRE(q_stride % 8 == 0 && out_stride % 8 == 0 && aligned16(q) && aligned16(out) && aligned16(scratch),
+               LCR_ERR_SHAPE, "chunk_attention needs 16-byte aligned rows and scratch");
+  LCRB_REQUIRE(static_cast<long long>(max_pages) * view->page_size <= INT32_MAX, LCR_ERR_SHAPE,
+               "chunk_attention: tables of %d pages of %d positions pass 31 bits", max_pages, view->page_size);
+  LCRB_REQUIRE(scratch_bytes >= lcr_chunk_attention_scratch_bytes(num_heads, view->head_dim), LCR_ERR_INVALID,
+               "chunk_attention: %zu bytes of scratch; it needs %zu", scratch_bytes,
+               lcr_chunk_attention_scratch_bytes(num_heads, view->head_dim));
+  ChunkAttnArgs a = {};
+  a.out = static_cast<bf16*>(out);
+  a.out_stride = out_stride;
+  a.q = static_cast<const bf16*>(q);
+  a.q_stride = q_stride;
+  a.keys = static_cast<const bf16*>(view->keys);
+  a.values = static_cast<const bf16*>(view->values);
+  a.tables = view->page_table;
+  a.max_pages = max_pages;
+  a.pool_pages = pool_pages;
+  a.page_size = view->page_size;
+  a.page_stride = view->page_stride;
+  a.head_stride = view->head_stride;
+  a.row_starts = row_starts;
+  a.kv_lengths = kv_lengths;
+  a.sequences = sequences;
+  a.rows = rows;
+  a.kv_heads = view->num_kv_heads;
+  a.group = num_heads / view->num_kv_heads;
+  a.scale_log2 = scale * kLog2e;
+  a.status = static_cast<uint32_t*>(scratch);
+  auto kernel = view->head_dim == 64 ? chunk_attn_kernel<64> : chunk_attn_kernel<128>;
+  const long long warps = static_cast<long long>(rows) * num_heads;
+  return launch_kernel(kernel, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, cs(stream), false, a);
+}
+
+extern "C" int lcr_chunk_attention_status(void* scratch, lcr_stream_t stream) {
+  LCRB_REQUIRE(scratch, LCR_ERR_INVALID, "chunk_attention_status: null scratch");
+  uint32_t st = 0;
+  LCRB_CUDA(cudaMemcpyAsync(&st, scratch, sizeof st, cudaMemcpyDeviceToHost, cs(stream)));
+  LCRB_CUDA(cudaStreamSynchronize(cs(stream)));
+  if (st == 0) return LCR_OK;
+  LCRB_CUDA(cudaMemsetAsync(scratch, 0, sizeof st, cs(stream)));
+  LCRB_CUDA(cudaStreamSynchronize(cs(stream)));
+  if (st & kStatusBadPage) return fail(LCR_ERR_POOL, "page table entry outside the pool (status 0x%x)", st);
+  return fail(LCR_ERR_TIMEOUT, "a device-side wait gave up (status 0x%x)", st);
+}
+
+extern "C" int lcr_token_probs(float* probs, int64_t probs_stride, const float* logits, int64_t logits_stride, int rows,
+                               int vocab, const float* temperature, const int32_t* row_sequence, lcr_stream_t stream) {
+  if (rows == 0) return LCR_OK;
+  LCRB_REQUIRE(probs && logits && rows > 0 && vocab > 0, LCR_ERR_INVALID, "token_probs: null pointer or bad size");
+  LCRB_REQUIRE(probs_stride >= vocab && logits_stride >= vocab, LCR_ERR_INVALID,
+               "token_probs: row strides %lld and %lld of %d ids", static_cast<long long>(probs_stride),
+               static_cast<long long>(logits_stride), vocab);
+  TokenProbsArgs a = {probs, probs_stride, logits, logits_stride, rows, vocab, temperature, row_sequence};
+  return launch_kernel(token_probs_kernel, dim3(static_cast<unsigned>(rows)), dim3(kProbsThreads), 0, cs(stream), false,
+                       a);
+}
+
+extern "C" int lcr_verify_drafts(int32_t* tokens, int32_t* accepted, const float* target_probs, int64_t target_stride,
+                                 const int32_t* target_starts, const int32_t* drafts, const int32_t* draft_counts,
+                                 const float* draft_probs, const float* uniforms, int sequences, int max_drafts,
+                                 int vocab, lcr_stream_t stream) {
+  if (sequences == 0) return LCR_OK;
+  LCRB_REQUIRE(tokens && accepted && target_probs && target_starts && draft_counts && uniforms && sequences > 0 &&
+                   max_drafts >= 0 && vocab > 0 && (max_drafts == 0 || drafts),
+               LCR_ERR_INVALID, "verify_drafts: null pointer or bad size");
+  LCRB_REQUIRE(target_stride >= vocab, LCR_ERR_INVALID, "verify_drafts: row stride %lld of %d ids",
+               static_cast<long long>(target_stride), vocab);
+  VerifyArgs a = {tokens,      accepted, target_probs, target_stride, target_starts, drafts, draft_counts,
+                  draft_probs, uniforms, sequences,    max_drafts,    vocab};
+  return launch_kernel(verify_drafts_kernel, dim3(static_cast<unsigned>(sequences)), dim3(kVerifyThreads), 0,
+                       cs(stream), false, a);
+}

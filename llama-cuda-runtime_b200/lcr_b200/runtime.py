@@ -101,6 +101,7 @@ class KvView(ctypes.Structure):
 _V = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
+_L = ctypes.c_int64
 _SIGS = {
     "lcr_last_error_string": (ctypes.c_char_p, []),
     "lcr_status_string": (ctypes.c_char_p, [_I]),
@@ -163,6 +164,14 @@ _SIGS = {
     "lcr_batch_stream": (_V, [_V]),
     "lcr_batch_step_launches": (_I, [_V, _I]),
     "lcr_batch_time_steps": (_I, [_V, _I, ctypes.POINTER(_F)]),
+    "lcr_plan_step": (_I, [_V, _I, _V, _V, _V, _V, _V, _I, _V, _V, _V, _I, _I, _I, _V, _V, _V, _V, _V, _V]),
+    "lcr_qk_norm_rope_kv": (_I, [_V, _L, ctypes.POINTER(KvView), _I, _V, _L, _I, _I, _V, _V, _F, _V, _V, _V, _V]),
+    "lcr_chunk_attention": (_I, [_V, _L, _V, _L, ctypes.POINTER(KvView), _I, _I, _V, _V, _I, _I, _I, _F, _V,
+                                 ctypes.c_size_t, _V]),
+    "lcr_chunk_attention_scratch_bytes": (ctypes.c_size_t, [_I, _I]),
+    "lcr_chunk_attention_status": (_I, [_V, _V]),
+    "lcr_token_probs": (_I, [_V, _L, _V, _L, _I, _I, _V, _V, _V]),
+    "lcr_verify_drafts": (_I, [_V, _V, _V, _L, _V, _V, _V, _V, _V, _I, _I, _I, _V]),
 }
 
 _lib: Optional[ctypes.CDLL] = None
