@@ -36,6 +36,27 @@ int check_view(const char* what, const lcr_kv_view* v, int pool_pages) {
   return LCR_OK;
 }
 
+// CTAs of the chunk attention (two per SM) on the current device; the
+// workspace holds a status word, a counter for each, and two parts for each.
+int attention_ctas() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    cudaGetLastError();
+    sms = 148;
+  }
+  return 2 * sms;
+}
+size_t attention_header(size_t ctas) { return 256 + (ctas * sizeof(unsigned) + 255) / 256 * 256; }
+
+template <int D>
+int launch_chunk_attention(const ChunkAttnArgs& a, int grid, cudaStream_t s) {
+  constexpr size_t smem = CaGeom<D>::SMEM;
+  LCRB_CUDA(cudaFuncSetAttribute(chunk_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(smem)));
+  return launch_kernel(chunk_attn_kernel<D>, dim3(static_cast<unsigned>(grid)), dim3(kCaThreads), smem, s, false, a);
+}
+
 }  // namespace
 
 extern "C" int lcr_plan_step(int32_t* block_tables, int max_pages, const int32_t* held, int32_t* held_out,
@@ -103,8 +124,8 @@ extern "C" int lcr_qk_norm_rope_kv(void* q_out, int64_t q_stride, const lcr_kv_v
 
 extern "C" size_t lcr_chunk_attention_scratch_bytes(int num_heads, int head_dim) {
   (void)num_heads;
-  (void)head_dim;
-  return 256;
+  const size_t ctas = static_cast<size_t>(attention_ctas());
+  return attention_header(ctas) + 2 * ctas * ca_part_floats(std::max(64, head_dim)) * sizeof(float);
 }
 
 extern "C" int lcr_chunk_attention(void* out, int64_t out_stride, const void* q, int64_t q_stride,
@@ -125,6 +146,11 @@ extern "C" int lcr_chunk_attention(void* out, int64_t out_stride, const void* q,
                static_cast<long long>(out_stride), static_cast<long long>(width));
   LCRB_REQUIRE(q_stride % 8 == 0 && out_stride % 8 == 0 && aligned16(q) && aligned16(out) && aligned16(scratch),
                LCR_ERR_SHAPE, "chunk_attention needs 16-byte aligned rows and scratch");
+  LCRB_REQUIRE(scale > 0.f && std::isfinite(scale), LCR_ERR_INVALID, "chunk_attention: scale %g must be positive",
+               static_cast<double>(scale));
+  LCRB_REQUIRE(static_cast<double>(pool_pages) * view->page_stride + static_cast<double>(view->num_kv_heads) * view->head_stride <
+                   34359738368.0,
+               LCR_ERR_SHAPE, "chunk_attention: a pool of more than 2^35 elements");
   LCRB_REQUIRE(static_cast<long long>(max_pages) * view->page_size <= INT32_MAX, LCR_ERR_SHAPE,
                "chunk_attention: tables of %d pages of %d positions pass 31 bits", max_pages, view->page_size);
   LCRB_REQUIRE(scratch_bytes >= lcr_chunk_attention_scratch_bytes(num_heads, view->head_dim), LCR_ERR_INVALID,
@@ -150,10 +176,19 @@ extern "C" int lcr_chunk_attention(void* out, int64_t out_stride, const void* q,
   a.kv_heads = view->num_kv_heads;
   a.group = num_heads / view->num_kv_heads;
   a.scale_log2 = scale * kLog2e;
-  a.status = static_cast<uint32_t*>(scratch);
-  auto kernel = view->head_dim == 64 ? chunk_attn_kernel<64> : chunk_attn_kernel<128>;
-  const long long warps = static_cast<long long>(rows) * num_heads;
-  return launch_kernel(kernel, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, cs(stream), false, a);
+  a.qb = kCaRows;
+  while (a.qb * a.group > kCaRows) a.qb /= 2;
+  const int ctas = attention_ctas();
+  char* work = static_cast<char*>(scratch);
+  a.status = reinterpret_cast<uint32_t*>(work);
+  a.counters = reinterpret_cast<unsigned*>(work + 256);
+  a.partials = reinterpret_cast<float*>(work + attention_header(static_cast<size_t>(ctas)));
+  // As many CTAs as the tables' capacity could give ranges.
+  const double tiles = static_cast<double>(a.kv_heads) * (static_cast<double>(rows) / a.qb + sequences);
+  const double blocks = tiles * ((static_cast<double>(max_pages) * a.page_size + rows) / kCaBlock + 1);
+  const int grid = static_cast<int>(std::min(static_cast<double>(ctas), std::max(1.0, blocks / kCaMinRange)));
+  return view->head_dim == 64 ? launch_chunk_attention<64>(a, grid, cs(stream))
+                              : launch_chunk_attention<128>(a, grid, cs(stream));
 }
 
 extern "C" int lcr_chunk_attention_status(void* scratch, lcr_stream_t stream) {
@@ -162,7 +197,8 @@ extern "C" int lcr_chunk_attention_status(void* scratch, lcr_stream_t stream) {
   LCRB_CUDA(cudaMemcpyAsync(&st, scratch, sizeof st, cudaMemcpyDeviceToHost, cs(stream)));
   LCRB_CUDA(cudaStreamSynchronize(cs(stream)));
   if (st == 0) return LCR_OK;
-  LCRB_CUDA(cudaMemsetAsync(scratch, 0, sizeof st, cs(stream)));
+  // A call that gave up may have left its counters up.
+  LCRB_CUDA(cudaMemsetAsync(scratch, 0, attention_header(static_cast<size_t>(attention_ctas())), cs(stream)));
   LCRB_CUDA(cudaStreamSynchronize(cs(stream)));
   if (st & kStatusBadPage) return fail(LCR_ERR_POOL, "page table entry outside the pool (status 0x%x)", st);
   return fail(LCR_ERR_TIMEOUT, "a device-side wait gave up (status 0x%x)", st);
