@@ -192,6 +192,54 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// Two bf16 in one conversion (the single conversions run on the
+// transcendental pipe, at an eighth of the rate).
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Pairs of fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// exp2_fma on a pair (2^x for x <= 8). x below -125, a masked key's -inf too,
+// counts as -125: a row that sees any key has a sum of at least 2^-8, beside
+// which 2^-125 is nothing, and ca_inverse tells a row that sees none by its
+// sum.
+__device__ __forceinline__ uint64_t exp2_fma2(float x, float y) {
+  const uint64_t v = pair(fmaxf(x, -125.0f), fmaxf(y, -125.0f));
+  const uint64_t t = add2(v, pair(12582912.0f, 12582912.0f));
+  const uint64_t n = add2(t, pair(-12582912.0f, -12582912.0f));
+  const uint64_t f = fma2(n, pair(-1.0f, -1.0f), v);
+  uint64_t p = pair(0.009569993242621422f, 0.009569993242621422f);
+  p = fma2(p, f, pair(0.055917542427778244f, 0.055917542427778244f));
+  p = fma2(p, f, pair(0.240247443318367f, 0.240247443318367f));
+  p = fma2(p, f, pair(0.6931218504905701f, 0.6931218504905701f));
+  p = fma2(p, f, pair(0.9999992847442627f, 0.9999992847442627f));
+  const float2 pf = unpair(p), tf = unpair(t);
+  return pair(__int_as_float(__float_as_int(pf.x) + (__float_as_int(tf.x) << 23)),
+              __int_as_float(__float_as_int(pf.y) + (__float_as_int(tf.y) << 23)));
+}
+
 // D (+)= A B with A in TMEM.
 __device__ __forceinline__ void tc_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b_desc, uint32_t idesc,
                                           uint32_t accumulate) {
@@ -212,6 +260,10 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&v)[32])
       "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
 }
+
+// 1 / l, 0 for a row that saw no key (whose l is at most 2^-125 for each
+// masked key), NaN for NaN.
+__device__ __forceinline__ float ca_inverse(float l) { return l > 1e-20f ? 1.0f / l : (l == l ? 0.f : l); }
 
 // Pair r of a split tile: the parts of ranges c0 .. c1 in that order.
 template <int D>
@@ -238,14 +290,14 @@ __device__ __forceinline__ void ca_join(const ChunkAttnArgs& a, long long c0, lo
         acc[4 * x + 3] = fmaf(v.w, wb, acc[4 * x + 3] * wa);
       }
     }
-    const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+    const float inv = ca_inverse(l);
     uint4* d4 = reinterpret_cast<uint4*>(dst + x0);
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
-      d4[x] = make_uint4(pack_bf2(acc[8 * x] * inv, acc[8 * x + 1] * inv),
-                         pack_bf2(acc[8 * x + 2] * inv, acc[8 * x + 3] * inv),
-                         pack_bf2(acc[8 * x + 4] * inv, acc[8 * x + 5] * inv),
-                         pack_bf2(acc[8 * x + 6] * inv, acc[8 * x + 7] * inv));
+      d4[x] = make_uint4(pack2(acc[8 * x] * inv, acc[8 * x + 1] * inv),
+                         pack2(acc[8 * x + 2] * inv, acc[8 * x + 3] * inv),
+                         pack2(acc[8 * x + 4] * inv, acc[8 * x + 5] * inv),
+                         pack2(acc[8 * x + 6] * inv, acc[8 * x + 7] * inv));
     }
   }
 }
@@ -550,11 +602,22 @@ __global__ void __launch_bounds__(kCaThreads, 2) chunk_attn_kernel(const ChunkAt
       const int pos = live ? w.q.kv - w.q.n + row : -1;  // keys 0 .. pos
       // The lowest position of the tile's rows: blocks that end below it need no mask.
       const int low = w.q.kv - w.q.n + w.t * a.qb;
+      // A warp without a live pair (a request of a few rows fills the first
+      // warp at most) only keeps the barriers going.
+      const bool idle = !__any_sync(0xffffffffu, live);
       float m = kNegBig, l = 0.f;
       for (int j = 0; j < cnt; ++j, ++g) {
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[g & 1], (g >> 1) & 1, a.status, kStatusTimeoutFull));
         if (!ok) break;
         tc_fence_after();
+        if (idle) {
+          if (j > 0) ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (g - 1) & 1, a.status, kStatusTimeoutFull));
+          if (!ok) break;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[g & 1]);
+          continue;
+        }
         const uint32_t tbuf = trow + (g & 1) * 64u;
         float s[64];
 #pragma unroll
@@ -585,20 +648,18 @@ __global__ void __launch_bounds__(kCaThreads, 2) chunk_attn_kernel(const ChunkAt
         const float na = grow ? top : m;
         const float alpha = ex2_approx(m - na);
         uint32_t pk[32];
-        float sums[8];
+        uint64_t sums[4] = {0, 0, 0, 0};
+        const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), shift2 = pair(-na, -na);
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          float p[8];
-#pragma unroll
-          for (int y = 0; y < 8; ++y) {
-            const float z = fmaf(s[8 * x + y], a.scale_log2, -na);
-            p[y] = x >= 8 - kCaFmaGroups ? exp2_fma(z) : ex2_approx(z);
-          }
-          sums[x] = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-#pragma unroll
-          for (int y = 0; y < 4; ++y) pk[4 * x + y] = pack_bf2(p[2 * y], p[2 * y + 1]);
+        for (int x = 0; x < 32; ++x) {
+          const float2 z = unpair(fma2(pair(s[2 * x], s[2 * x + 1]), scale2, shift2));
+          const uint64_t p = (x & 7) >= 8 - kCaFmaGroups ? exp2_fma2(z.x, z.y) : pair(ex2_approx(z.x), ex2_approx(z.y));
+          sums[x & 3] = add2(sums[x & 3], p);
+          const float2 pf = unpair(p);
+          pk[x] = pack2(pf.x, pf.y);
         }
-        l = fmaf(l, alpha, ((sums[0] + sums[1]) + (sums[2] + sums[3])) + ((sums[4] + sums[5]) + (sums[6] + sums[7])));
+        const float2 sum = unpair(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+        l = fmaf(l, alpha, sum.x + sum.y);
         m = na;
         tc_st32(tbuf, pk);
         if (j > 0) {
@@ -631,7 +692,7 @@ __global__ void __launch_bounds__(kCaThreads, 2) chunk_attn_kernel(const ChunkAt
       tc_fence_after();
       bf16* dst = a.out + (live ? (w.q.row0 + row) * a.out_stride + head : 0);
       if (cnt == w.len) {
-        const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays
+        const float inv = ca_inverse(l);
 #pragma unroll
         for (int x = 0; x < D; x += 16) {
           float o[16];
@@ -641,9 +702,9 @@ __global__ void __launch_bounds__(kCaThreads, 2) chunk_attn_kernel(const ChunkAt
             uint4* d4 = reinterpret_cast<uint4*>(dst + x);
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-              d4[y] = make_uint4(pack_bf2(o[8 * y] * inv, o[8 * y + 1] * inv), pack_bf2(o[8 * y + 2] * inv, o[8 * y + 3] * inv),
-                                 pack_bf2(o[8 * y + 4] * inv, o[8 * y + 5] * inv),
-                                 pack_bf2(o[8 * y + 6] * inv, o[8 * y + 7] * inv));
+              d4[y] = make_uint4(pack2(o[8 * y] * inv, o[8 * y + 1] * inv), pack2(o[8 * y + 2] * inv, o[8 * y + 3] * inv),
+                                 pack2(o[8 * y + 4] * inv, o[8 * y + 5] * inv),
+                                 pack2(o[8 * y + 6] * inv, o[8 * y + 7] * inv));
             }
           }
         }
