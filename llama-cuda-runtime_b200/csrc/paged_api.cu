@@ -36,16 +36,16 @@ int check_view(const char* what, const lcr_kv_view* v, int pool_pages) {
   return LCR_OK;
 }
 
-// CTAs of the chunk attention (two per SM) on the current device; the
-// workspace holds a status word, a counter for each, and two parts for each.
-int attention_ctas() {
+// CTAs of the chunk attention on the current device; the workspace holds a
+// status word, a counter for each, and two parts for each.
+int attention_ctas(int head_dim) {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
     cudaGetLastError();
     sms = 148;
   }
-  return 2 * sms;
+  return (head_dim == 64 ? CaGeom<64>::CTAS : CaGeom<128>::CTAS) * sms;
 }
 size_t attention_header(size_t ctas) { return 256 + (ctas * sizeof(unsigned) + 255) / 256 * 256; }
 
@@ -124,7 +124,7 @@ extern "C" int lcr_qk_norm_rope_kv(void* q_out, int64_t q_stride, const lcr_kv_v
 
 extern "C" size_t lcr_chunk_attention_scratch_bytes(int num_heads, int head_dim) {
   (void)num_heads;
-  const size_t ctas = static_cast<size_t>(attention_ctas());
+  const size_t ctas = static_cast<size_t>(attention_ctas(head_dim));
   return attention_header(ctas) + 2 * ctas * ca_part_floats(std::max(64, head_dim)) * sizeof(float);
 }
 
@@ -176,16 +176,27 @@ extern "C" int lcr_chunk_attention(void* out, int64_t out_stride, const void* q,
   a.kv_heads = view->num_kv_heads;
   a.group = num_heads / view->num_kv_heads;
   a.scale_log2 = scale * kLog2e;
-  a.qb = kCaRows;
-  while (a.qb * a.group > kCaRows) a.qb /= 2;
-  const int ctas = attention_ctas();
+  a.log2_qb = 7;
+  while (a.log2_qb > 0 && (a.group << a.log2_qb) > kCaRows) --a.log2_qb;
+  // Division by the page size: with 2^s >= page_size, mul = ceil(2^(31 + s) /
+  // page_size) is exact for keys below 2^31.
+  int s = 0;
+  while ((1ll << s) < view->page_size) ++s;
+  if (s > 0) {
+    a.page_shift = static_cast<unsigned>(s - 1);
+    a.page_mul = static_cast<unsigned>(((1ull << (31 + s)) + view->page_size - 1) / view->page_size);
+  }
+  const int ctas = attention_ctas(view->head_dim);
   char* work = static_cast<char*>(scratch);
   a.status = reinterpret_cast<uint32_t*>(work);
   a.counters = reinterpret_cast<unsigned*>(work + 256);
   a.partials = reinterpret_cast<float*>(work + attention_header(static_cast<size_t>(ctas)));
   // As many CTAs as the tables' capacity could give ranges.
-  const double tiles = static_cast<double>(a.kv_heads) * (static_cast<double>(rows) / a.qb + sequences);
-  const double blocks = tiles * ((static_cast<double>(max_pages) * a.page_size + rows) / kCaBlock + 1);
+  const double tiles = a.kv_heads * (std::ldexp(static_cast<double>(rows), -a.log2_qb) + sequences);
+  const double blocks = tiles * ((static_cast<double>(max_pages) * view->page_size + rows) / view->head_dim + 1);
+  LCRB_REQUIRE(blocks < 2147483647.0, LCR_ERR_SHAPE,
+               "chunk_attention: %d rows of %d requests over tables of %d positions are too many blocks", rows, sequences,
+               max_pages * view->page_size);
   const int grid = static_cast<int>(std::min(static_cast<double>(ctas), std::max(1.0, blocks / kCaMinRange)));
   return view->head_dim == 64 ? launch_chunk_attention<64>(a, grid, cs(stream))
                               : launch_chunk_attention<128>(a, grid, cs(stream));
@@ -198,7 +209,7 @@ extern "C" int lcr_chunk_attention_status(void* scratch, lcr_stream_t stream) {
   LCRB_CUDA(cudaStreamSynchronize(cs(stream)));
   if (st == 0) return LCR_OK;
   // A call that gave up may have left its counters up.
-  LCRB_CUDA(cudaMemsetAsync(scratch, 0, attention_header(static_cast<size_t>(attention_ctas())), cs(stream)));
+  LCRB_CUDA(cudaMemsetAsync(scratch, 0, attention_header(static_cast<size_t>(attention_ctas(64))), cs(stream)));
   LCRB_CUDA(cudaStreamSynchronize(cs(stream)));
   if (st & kStatusBadPage) return fail(LCR_ERR_POOL, "page table entry outside the pool (status 0x%x)", st);
   return fail(LCR_ERR_TIMEOUT, "a device-side wait gave up (status 0x%x)", st);
