@@ -36,12 +36,13 @@
 // counter per split tile) joins them in range order, so the result does not
 // depend on which one that is.
 //
-// Loads. Pages may have any size and any strides, so K and V rows are fetched
-// 16 bytes at a time (cp.async) by one warp, each lane holding the cache rows
-// of its keys, into a ring of 128-byte wide panels in the swizzled layout;
-// keys past the tile's last position are filled with zeros and their pages
-// never looked up, so what lies there cannot reach the sums. The ring runs
-// ahead across tiles.
+// Loads. One warp fills a ring of 128-byte wide panels of K and V in the
+// swizzled layout, ahead across tiles. Where the pool is dense and a page holds
+// a multiple of 16 positions, by tensor copies of 16 to 128 keys; else 16 bytes
+// at a time (cp.async), each lane holding the cache rows of its keys: any page
+// size and strides, but the issue of a copy costs the warp about 15 cycles, and
+// it bounds the kernel (LOADS). Keys past the tile's last position are never
+// read and enter as zeros, so what lies there cannot reach the sums.
 //
 // Warps: 0-3 softmax (warp w owns TMEM lanes 32 w .. + 31) and epilogue, 4
 // TMEM allocation and MMA issue, 5 loads. Every wait is bounded.
@@ -55,7 +56,8 @@ namespace lcrb {
 
 constexpr int kCaThreads = 192;
 constexpr int kCaRows = 128;      // (row, head) pairs per tile
-constexpr int kCaMinRange = 2;    // blocks a CTA takes at least (where there are as many)
+constexpr int kCaTileCost = 2;    // units a tile's start and end count for, beside one for each block
+constexpr int kCaMinRange = 4;    // units a CTA takes at least (where there are as many)
 constexpr int kCaFmaGroups = 1;   // of 8 pairs of exponentials, on the FMA pipe
 
 struct ChunkAttnArgs {
@@ -72,6 +74,8 @@ struct ChunkAttnArgs {
   const int32_t* kv_lengths;
   int sequences, rows, kv_heads, group;
   int log2_qb;          // rows per tile: 2^log2_qb
+  int log2_unit;        // keys per tensor copy: 2^log2_unit, at most a page and a block
+  int pool_rows;        // rows of head_dim in a pool (tensor copies)
   unsigned page_mul, page_shift;  // key / page_size = umulhi(key, page_mul) >> page_shift (page_size > 1)
   float scale_log2;
   uint32_t* status;
@@ -115,6 +119,15 @@ __device__ __forceinline__ int ca_blocks_before(int s, int t, int log2_qb) {
   return static_cast<int>(below(a1 + n + 1) - below(a1 + 1));
 }
 
+// Ranges are cut in units of blocks with kCaTileCost units added in front of
+// every tile, about what a change of tiles costs (Q, the first S, the
+// epilogue): a range with many short tiles gets fewer blocks.
+
+template <int BLK>
+__device__ __forceinline__ int ca_units_before(int s, int t, int log2_qb) {
+  return ca_blocks_before<BLK>(s, t, log2_qb) + t * kCaTileCost;
+}
+
 // One request as the kernel sees it: malformed lengths are cut to what the
 // arrays hold.
 struct CaSeq {
@@ -122,7 +135,7 @@ struct CaSeq {
   int kv;       // cached positions
   int s;        // max(0, kv - n): where the block count starts
   int tiles;
-  int blocks;   // of one KV head
+  int units;    // of one KV head
 };
 
 template <int BLK>
@@ -133,7 +146,8 @@ __device__ __forceinline__ CaSeq ca_seq(const ChunkAttnArgs& a, int b) {
   q.kv = min(max(0, a.kv_lengths[b]), a.max_pages * a.page_size);
   q.s = max(0, q.kv - q.n);
   q.tiles = (q.n + (1 << a.log2_qb) - 1) >> a.log2_qb;
-  q.blocks = q.tiles == 0 ? 0 : ca_blocks_before<BLK>(q.s, q.tiles - 1, a.log2_qb) + (q.s + q.n + BLK - 1) / BLK;
+  q.units = q.tiles == 0 ? 0
+                         : ca_units_before<BLK>(q.s, q.tiles - 1, a.log2_qb) + (q.s + q.n + BLK - 1) / BLK + kCaTileCost;
   return q;
 }
 
@@ -142,46 +156,52 @@ __device__ __forceinline__ int ca_tile_len(const CaSeq& q, int t, int log2_qb) {
   return (q.s + min(q.n, (t + 1) << log2_qb) + BLK - 1) / BLK;
 }
 
-// A CTA's walk over its range of blocks, segment by segment (a segment = its
-// share of one tile). Every warp walks for itself.
+// A CTA's walk over its range of units, segment by segment (a segment = its
+// share of one tile, in whole blocks). Every warp walks for itself.
 template <int BLK>
 struct CaWalk {
   int b, h, t;
   CaSeq q;
   int len;   // blocks of the tile
-  int off;   // first block of this segment
-  int left;  // blocks of the range from here on
+  int at;    // units of the tile before this segment
+  int left;  // units of the range from here on
 
-  // To block `at` of request b.
-  __device__ __forceinline__ void find(const ChunkAttnArgs& a, int b0, int at) {
+  // To unit `from` of request b0's.
+  __device__ __forceinline__ void find(const ChunkAttnArgs& a, int b0, int from) {
     b = b0;
     q = ca_seq<BLK>(a, b);
-    h = at / q.blocks;
-    const int rem = at - h * q.blocks;
+    h = from / q.units;
+    const int rem = from - h * q.units;
     int lo = 0, hi = q.tiles - 1;  // the last tile that begins at or before rem
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (ca_blocks_before<BLK>(q.s, mid, a.log2_qb) <= rem) lo = mid;
+      if (ca_units_before<BLK>(q.s, mid, a.log2_qb) <= rem) lo = mid;
       else hi = mid - 1;
     }
     t = lo;
-    off = rem - ca_blocks_before<BLK>(q.s, t, a.log2_qb);
+    at = rem - ca_units_before<BLK>(q.s, t, a.log2_qb);
   }
-  __device__ __forceinline__ void open(const ChunkAttnArgs& a, int b0, int h0, int t0, int off0, int count) {
+  __device__ __forceinline__ void open(const ChunkAttnArgs& a, int b0, int h0, int t0, int at0, int units) {
     b = b0;
     h = h0;
     t = t0;
-    off = off0;
-    left = count;
+    at = at0;
+    left = units;
     q = ca_seq<BLK>(a, b);
     len = ca_tile_len<BLK>(q, t, a.log2_qb);
   }
-  __device__ __forceinline__ int count() const { return min(len - off, left); }
+  __device__ __forceinline__ int units() const { return min(len + kCaTileCost - at, left); }
+  __device__ __forceinline__ int off() const { return max(0, at - kCaTileCost); }  // first block of the segment
+  __device__ __forceinline__ int count() const { return max(0, at + units() - kCaTileCost) - off(); }  // its blocks
+  // Keys the tile's last row sees, of those cached.
+  __device__ __forceinline__ int key_end(const ChunkAttnArgs& a) const {
+    return max(0, q.kv - q.n + min(q.n, (t + 1) << a.log2_qb));
+  }
   // Past this segment; false at the end of the range.
   __device__ __forceinline__ bool next(const ChunkAttnArgs& a) {
-    left -= count();
+    left -= units();
     if (left <= 0) return false;
-    off = 0;
+    at = 0;
     if (++t == q.tiles) {
       t = 0;
       if (++h == a.kv_heads) {
@@ -266,6 +286,15 @@ __device__ __forceinline__ uint64_t exp2_fma2(float x, float y) {
   const float2 pf = unpair(p), tf = unpair(t);
   return pair(__int_as_float(__float_as_int(pf.x) + (__float_as_int(tf.x) << 23)),
               __int_as_float(__float_as_int(pf.y) + (__float_as_int(tf.y) << 23)));
+}
+
+// One tensor copy: rows `row` .. of a pool, 64 columns of panel `panel`.
+__device__ __forceinline__ void ca_tma(uint32_t dst, const CUtensorMap* map, int row, int panel, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+          "r"(dst),
+      "l"(map), "r"(0), "r"(row), "r"(panel), "r"(smem_addr(bar))
+      : "memory");
 }
 
 // D (+)= A B with A in TMEM.
@@ -358,8 +387,10 @@ __device__ __forceinline__ void ca_join(const ChunkAttnArgs& a, int c0, int c1, 
   }
 }
 
-template <int D>
-__global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel(const ChunkAttnArgs a) {
+template <int D, bool TMA>
+__global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel(const ChunkAttnArgs a,
+                                                                                const __grid_constant__ CUtensorMap kmap,
+                                                                                const __grid_constant__ CUtensorMap vmap) {
   using G = CaGeom<D>;
   constexpr int SLOTS = G::SLOTS, BLOCK = G::BLOCK;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -402,17 +433,17 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
     mbar_fence_init();
   }
 
-  // --- This CTA's range of blocks --------------------------------------------
+  // --- This CTA's range of units --------------------------------------------
   // Scratch of the scan, in the ring before its first use.
   struct Start {
     int part[kCaThreads / 32];
-    int b, h, t, off;
+    int b, h, t, at;
   };
   Start* st = reinterpret_cast<Start*>(ring);
   const int per_thread = (a.sequences + kCaThreads - 1) / kCaThreads;
   const int b0 = min(a.sequences, tid * per_thread), b1 = min(a.sequences, b0 + per_thread);
   int mine = 0;
-  for (int b = b0; b < b1; ++b) mine += ca_seq<BLOCK>(a, b).blocks * a.kv_heads;
+  for (int b = b0; b < b1; ++b) mine += ca_seq<BLOCK>(a, b).units * a.kv_heads;
   int incl = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -438,7 +469,7 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
   const int lo = some ? c * per : total, hi = min(total - lo, per) + lo;
   if (lo >= before && lo < before + mine) {
     int at = lo - before, b = b0;
-    for (int n = ca_seq<BLOCK>(a, b).blocks * a.kv_heads; at >= n; n = ca_seq<BLOCK>(a, b).blocks * a.kv_heads) {
+    for (int n = ca_seq<BLOCK>(a, b).units * a.kv_heads; at >= n; n = ca_seq<BLOCK>(a, b).units * a.kv_heads) {
       at -= n;
       ++b;
     }
@@ -447,22 +478,99 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
     st->b = w.b;
     st->h = w.h;
     st->t = w.t;
-    st->off = w.off;
+    st->at = w.at;
   }
   __syncthreads();
-  const int start_b = st->b, start_h = st->h, start_t = st->t, start_off = st->off;
+  const int start_b = st->b, start_h = st->h, start_t = st->t, start_at = st->at;
   __syncthreads();  // the scratch becomes the ring
 
   const uint32_t tmem = *tmem_slot;
   const bool aligned = (smem_addr(smem) & 1023u) == 0;
   if (!aligned && tid == 0) atomicOr(a.status, kStatusBadSmem | kStatusAbort);
   CaWalk<BLOCK> w;
-  if (some) w.open(a, start_b, start_h, start_t, start_off, hi - lo);
+  if (some) w.open(a, start_b, start_h, start_t, start_at, hi - lo);
 
   if (!aligned || !some) {
     // Nothing is in flight.
+  } else if (warp == 5 && TMA) {
+    // --- Loads by tensor copies ----------------------------------------------
+    // A slot's keys come in units that lie within a page: lane u looks up unit
+    // u of a block (one block ahead) and lane 0 copies it. The keys of the
+    // unit that the tile's last position ends in are copied one by one, zeros
+    // after them up to a multiple of 16: the MMA warp uses no later ones.
+    int issued = 0;  // slots (the panels of a block's K, of its V, ...) issued
+    bool ok = true;
+    const uint32_t ring_addr = smem_addr(ring);
+    auto page_of = [&](int key) { return static_cast<int>(__umulhi(static_cast<unsigned>(key), a.page_mul) >> a.page_shift); };
+    const bool leader = elect_one();
+    if (leader) {
+      prefetch_tensormap(&kmap);
+      prefetch_tensormap(&vmap);
+    }
+    do {
+      const int cnt = w.count(), off = w.off(), key_end = w.key_end(a);
+      const int32_t* table = a.tables + static_cast<size_t>(w.b) * a.max_pages;
+      int page = -1;
+      auto look = [&](int j) {
+        const int key = j * BLOCK + (lane << a.log2_unit);
+        page = lane < (BLOCK >> a.log2_unit) && key < key_end ? __ldg(table + page_of(key)) : -1;
+      };
+      if (cnt > 0) look(off);
+      for (int j = off; j < off + cnt && ok; ++j) {
+        // This lane's unit as a row of the pool; past its end (which reads as
+        // zeros) for a page outside it.
+        const int key = j * BLOCK + (lane << a.log2_unit);
+        const bool in = page >= 0 && page < a.pool_pages;
+        if (!in && lane < (BLOCK >> a.log2_unit) && key < key_end) atomicOr(a.status, kStatusBadPage);
+        const int row = in ? (page * a.kv_heads + w.h) * a.page_size + key - page_of(key) * a.page_size : a.pool_rows;
+        if (j + 1 < off + cnt) look(j + 1);
+        const int live = min(max(key_end - j * BLOCK, 0), BLOCK);
+        const int units = live >> a.log2_unit;
+        const int done = units << a.log2_unit, rest = max(16, (live + 15) & ~15) - done;  // rest < 0: the block is full
+        const int last = __shfl_sync(0xffffffffu, row, units & 31);
+        int at[BLOCK / 16];
+#pragma unroll
+        for (int u = 0; u < BLOCK / 16; ++u) at[u] = __shfl_sync(0xffffffffu, row, u);
+#pragma unroll 1
+        for (int x = 0; x < 2 * G::PANELS; ++x) {  // K's panels, then V's
+          const int slot = issued % SLOTS;
+          if (issued >= SLOTS) ok = ca_wait(&empty[slot], ((issued / SLOTS) - 1) & 1, a.status, kStatusTimeoutEmpty);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const uint32_t dst = ring_addr + slot * G::SLOT;
+          const int panel = x % G::PANELS;
+          // Unrolled, so that the copies' operands reach uniform registers
+          // side by side (in a loop a copy took 170 cycles).
+          if (leader) {
+#pragma unroll
+            for (int u = 0; u < BLOCK / 16; ++u) {
+              if (u < units) ca_tma(dst + (u << a.log2_unit) * 128, x < G::PANELS ? &kmap : &vmap, at[u], panel, &full[slot]);
+            }
+          }
+          if (rest > 0) {
+            const uint4* base = reinterpret_cast<const uint4*>(x < G::PANELS ? a.keys : a.values) + panel * 8 + (lane & 7);
+            for (int r = lane >> 3; r < rest; r += 4) {
+              const bool in = done + r < live && last < a.pool_rows;
+              const int key = done + r;
+              cp_async16(dst + key * 128 + (((lane & 7) ^ (key & 7)) << 4),
+                         base + (in ? static_cast<long long>(last + r) * (D / 8) : 0ll), in);
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (leader) mbar_arrive_expect_tx(&full[slot], static_cast<uint32_t>(done) * 128);
+          ++issued;
+        }
+      }
+    } while (ok && w.next(a));
+    // Copies in flight land before the CTA ends.
+    if (!ok && lane == 0) {
+      for (int i = max(0, issued - SLOTS); i < issued; ++i) mbar_wait(&full[i % SLOTS], (i / SLOTS) & 1, nullptr, 0);
+    }
   } else if (warp == 5) {
-    // --- Loads ---------------------------------------------------------------
+    // --- Loads row by row ----------------------------------------------------
     constexpr int LOOK = BLOCK / 32;  // lane l looks up keys l, l + 32, ... of a block
     int issued = 0;                   // slots (the panels of a block's K, of its V, ...) issued
     bool ok = true;
@@ -476,8 +584,7 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
     const uint32_t ring_addr = smem_addr(ring);
     do {
       const int cnt = w.count();
-      // Keys the tile's last row sees, of those cached.
-      const int key_end = max(0, w.q.kv - w.q.n + min(w.q.n, (w.t + 1) << a.log2_qb));
+      const int key_end = w.key_end(a), off = w.off();
       const int32_t* table = a.tables + static_cast<size_t>(w.b) * a.max_pages;
       const long long head = w.h * a.head_stride;
       auto page_of = [&](int key) {
@@ -493,8 +600,8 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
           page[i] = key < key_end ? __ldg(table + page_of(key)) : -1;
         }
       };
-      look(w.off);
-      for (int j = w.off; j < w.off + cnt && ok; ++j) {
+      if (cnt > 0) look(off);
+      for (int j = off; j < off + cnt && ok; ++j) {
         uint32_t row[LOOK];  // cache rows of this lane's keys, in 16-byte units; ~0u: zeros
 #pragma unroll
         for (int i = 0; i < LOOK; ++i) {
@@ -504,7 +611,7 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
           const long long slot = key - page_of(key) * a.page_size;
           row[i] = in ? static_cast<uint32_t>((page[i] * a.page_stride + head + slot * D) >> 3) : 0xffffffffu;
         }
-        if (j + 1 < w.off + cnt) look(j + 1);
+        if (j + 1 < off + cnt) look(j + 1);
 #pragma unroll 1
         for (int x = 0; x < 2 * G::PANELS; ++x) {  // K's panels, then V's
           const int slot = issued % SLOTS;
@@ -559,7 +666,8 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
     uint32_t tile = 0;
     bool ok = true;
     do {
-      const int cnt = w.count();
+      const int cnt = w.count(), off = w.off(), key_end = w.key_end(a);
+      if (cnt == 0) continue;
       ok = wait(q_full, tile & 1);
       for (int j = 0; j < cnt && ok; ++j, ++g) {
         // K, then P V of the block before: S goes over its P.
@@ -597,7 +705,10 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
         if (leader) {
 #pragma unroll
           for (int k = 0; k < BLOCK / 16; ++k) {
-            tc_mma_ts(base + G::O_COL, base + k * 8u, vdesc + k * 2048 / 16, idesc_pv, j + k > 0 ? 1u : 0u);
+            // (Keys that no row sees weigh nothing.)
+            if (k == 0 || (off + j) * BLOCK + 16 * k < key_end) {
+              tc_mma_ts(base + G::O_COL, base + k * 8u, vdesc + k * 2048 / 16, idesc_pv, j + k > 0 ? 1u : 0u);
+            }
           }
 #pragma unroll
           for (int p = 0; p < G::PANELS; ++p) tc_commit(&empty[v0 + p]);
@@ -619,9 +730,13 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
     int g = 0;
     bool ok = true;
     int parts = 0;        // parts stored so far
-    int done = lo;        // blocks of all tiles before this segment
+    int done = lo;        // units before this segment
     do {
-      const int cnt = w.count();
+      const int cnt = w.count(), off = w.off();
+      if (cnt == 0) {
+        done += w.units();
+        continue;
+      }
       const int row = (w.t << a.log2_qb) + qi;  // of the request
       const bool live = qi < (1 << a.log2_qb) && row < w.q.n;
       const long long head = static_cast<long long>(w.h * a.group + hl) * D;
@@ -668,8 +783,8 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
           if (lane == 0) mbar_arrive(p_full);
           continue;
         }
-        const int lim = pos - (w.off + j) * BLOCK;  // keys of the block past it are masked
-        const bool masked = (w.off + j + 1) * BLOCK - 1 > low;
+        const int lim = pos - (off + j) * BLOCK;  // keys of the block past it are masked
+        const bool masked = (off + j + 1) * BLOCK - 1 > low;
         float v[32];
         auto fetch = [&](int c) {
           tc_ld32(trow + 32 * c, v);
@@ -755,8 +870,8 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
       } else {
         // A part: columns of four as [column / 4][pair], so neighbouring
         // threads' 16 bytes are neighbours.
-        const int tile0 = done - w.off;
-        float* part = a.partials + static_cast<size_t>(2 * c + (w.off > 0 ? 0 : 1)) * ca_part_floats(D);
+        const int tile0 = done - w.at + kCaTileCost;  // unit of the tile's first block
+        float* part = a.partials + static_cast<size_t>(2 * c + (off > 0 ? 0 : 1)) * ca_part_floats(D);
         if (live) {
           part[r] = m;
           part[kCaRows + r] = l;
@@ -794,7 +909,7 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
         if (*last_s && live) ca_join<D>(a, c0, c1, r, dst);
       }
       tc_fence_before();  // O and S were read: the next tile's MMAs may write them
-      done += cnt;
+      done += w.units();
     } while (w.next(a));
   }
   tc_fence_before();

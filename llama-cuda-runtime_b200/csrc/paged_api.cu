@@ -10,6 +10,7 @@
 #include "lcr_b200.h"
 #include "qk_norm_rope.cuh"
 #include "step_plan.cuh"
+#include "tmap.h"
 #include "token_probs.cuh"
 #include "verify_drafts.cuh"
 
@@ -49,12 +50,30 @@ int attention_ctas(int head_dim) {
 }
 size_t attention_header(size_t ctas) { return 256 + (ctas * sizeof(unsigned) + 255) / 256 * 256; }
 
-template <int D>
-int launch_chunk_attention(const ChunkAttnArgs& a, int grid, cudaStream_t s) {
+template <int D, bool TMA>
+int launch_chunk_attention(const ChunkAttnArgs& a, const CUtensorMap& kmap, const CUtensorMap& vmap, int grid,
+                           cudaStream_t s) {
   constexpr size_t smem = CaGeom<D>::SMEM;
-  LCRB_CUDA(cudaFuncSetAttribute(chunk_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(smem)));
-  return launch_kernel(chunk_attn_kernel<D>, dim3(static_cast<unsigned>(grid)), dim3(kCaThreads), smem, s, false, a);
+  auto kernel = chunk_attn_kernel<D, TMA>;
+  LCRB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  return launch_kernel(kernel, dim3(static_cast<unsigned>(grid)), dim3(kCaThreads), smem, s, false, a, kmap, vmap);
+}
+
+template <int D>
+int chunk_attention(ChunkAttnArgs& a, int grid, cudaStream_t s) {
+  CUtensorMap kmap = {}, vmap = {};
+  const long long rows = static_cast<long long>(a.pool_pages) * a.kv_heads * a.page_size;
+  // Tensor copies see a pool as rows of head_dim, and a copy lies within a page.
+  const bool dense = a.head_stride == static_cast<long long>(a.page_size) * D && a.page_stride == a.kv_heads * a.head_stride;
+  if (dense && a.page_size % 16 == 0 && rows < INT32_MAX) {
+    a.log2_unit = 4;
+    while ((2 << a.log2_unit) <= CaGeom<D>::BLOCK && a.page_size % (2 << a.log2_unit) == 0) ++a.log2_unit;
+    a.pool_rows = static_cast<int>(rows);
+    LCRB_TRY(make_kmajor_map(&kmap, a.keys, a.pool_rows, D, 1, 1 << a.log2_unit, 1));
+    LCRB_TRY(make_kmajor_map(&vmap, a.values, a.pool_rows, D, 1, 1 << a.log2_unit, 1));
+    return launch_chunk_attention<D, true>(a, kmap, vmap, grid, s);
+  }
+  return launch_chunk_attention<D, false>(a, kmap, vmap, grid, s);
 }
 
 }  // namespace
@@ -193,13 +212,12 @@ extern "C" int lcr_chunk_attention(void* out, int64_t out_stride, const void* q,
   a.partials = reinterpret_cast<float*>(work + attention_header(static_cast<size_t>(ctas)));
   // As many CTAs as the tables' capacity could give ranges.
   const double tiles = a.kv_heads * (std::ldexp(static_cast<double>(rows), -a.log2_qb) + sequences);
-  const double blocks = tiles * ((static_cast<double>(max_pages) * view->page_size + rows) / view->head_dim + 1);
+  const double blocks = tiles * ((static_cast<double>(max_pages) * view->page_size + rows) / view->head_dim + 1 + kCaTileCost);
   LCRB_REQUIRE(blocks < 2147483647.0, LCR_ERR_SHAPE,
                "chunk_attention: %d rows of %d requests over tables of %d positions are too many blocks", rows, sequences,
                max_pages * view->page_size);
   const int grid = static_cast<int>(std::min(static_cast<double>(ctas), std::max(1.0, blocks / kCaMinRange)));
-  return view->head_dim == 64 ? launch_chunk_attention<64>(a, grid, cs(stream))
-                              : launch_chunk_attention<128>(a, grid, cs(stream));
+  return view->head_dim == 64 ? chunk_attention<64>(a, grid, cs(stream)) : chunk_attention<128>(a, grid, cs(stream));
 }
 
 extern "C" int lcr_chunk_attention_status(void* scratch, lcr_stream_t stream) {
