@@ -56,8 +56,9 @@ namespace lcrb {
 
 constexpr int kCaThreads = 192;
 constexpr int kCaRows = 128;      // (row, head) pairs per tile
-constexpr int kCaTileCost = 2;    // units a tile's start and end count for, beside one for each block
-constexpr int kCaMinRange = 4;    // units a CTA takes at least (where there are as many)
+constexpr int kCaTileCost = 3;    // units a tile's start and end count for, beside one for each block
+constexpr int kCaSnap = 4;        // units from a tile's end within which a range's end moves there
+constexpr int kCaMinRange = 4;    // units of a range at least (where there are as many); at least kCaSnap
 constexpr int kCaFmaGroups = 1;   // of 8 pairs of exponentials, on the FMA pipe
 
 struct ChunkAttnArgs {
@@ -180,6 +181,7 @@ struct CaWalk {
     }
     t = lo;
     at = rem - ca_units_before<BLK>(q.s, t, a.log2_qb);
+    len = ca_tile_len<BLK>(q, t, a.log2_qb);
   }
   __device__ __forceinline__ void open(const ChunkAttnArgs& a, int b0, int h0, int t0, int at0, int units) {
     b = b0;
@@ -197,10 +199,8 @@ struct CaWalk {
   __device__ __forceinline__ int key_end(const ChunkAttnArgs& a) const {
     return max(0, q.kv - q.n + min(q.n, (t + 1) << a.log2_qb));
   }
-  // Past this segment; false at the end of the range.
-  __device__ __forceinline__ bool next(const ChunkAttnArgs& a) {
-    left -= units();
-    if (left <= 0) return false;
+  // To the start of the next tile (there is one).
+  __device__ __forceinline__ void advance(const ChunkAttnArgs& a) {
     at = 0;
     if (++t == q.tiles) {
       t = 0;
@@ -212,9 +212,30 @@ struct CaWalk {
       }
     }
     len = ca_tile_len<BLK>(q, t, a.log2_qb);
+  }
+  // Past this segment; false at the end of the range.
+  __device__ __forceinline__ bool next(const ChunkAttnArgs& a) {
+    left -= units();
+    if (left <= 0) return false;
+    advance(a);
     return true;
   }
 };
+
+// How far an end of a range that lies `at` units into a tile of `units` moves:
+// splitting a tile costs its CTAs about as much as kCaSnap units (a part stored,
+// counted and joined). Ends are at least kCaSnap apart, so that only one of a
+// tile's moves to each of its own ends.
+__device__ __forceinline__ int ca_snap(int at, int units) {
+  return at <= kCaSnap ? -at : units - at <= kCaSnap ? units - at : 0;
+}
+// The range that unit `y` of the tile [begin, begin + units) falls to.
+__device__ __forceinline__ int ca_owner(int y, int begin, int units, int per) {
+  const int c = y / per, from = c * per - begin, to = from + per;
+  if (from > 0 && ca_snap(from, units) > 0) return c - 1;
+  if (to < units && ca_snap(to, units) < 0) return c + 1;
+  return c;
+}
 
 // mbar_wait with its slow path out of line: the kernel waits in many places,
 // and its loops should stay within the instruction caches.
@@ -350,40 +371,84 @@ constexpr uint32_t ca_idesc(int n) {
 // masked key), NaN for NaN.
 __device__ __forceinline__ float ca_inverse(float l) { return l > 1e-20f ? 1.0f / l : (l == l ? 0.f : l); }
 
-// Pair r of a split tile: the parts of ranges c0 .. c1 in that order.
+// 32 scores of this lane, those past column lim masked.
+__device__ __forceinline__ void ca_fetch(uint32_t taddr, float (&v)[32], bool masked, int lim) {
+  tc_ld32(taddr, v);
+  tc_wait_ld();
+  if (masked) {
+    asm volatile("" ::: "memory");  // a branch, not 32 predicated selects in every block
+#pragma unroll
+    for (int x = 0; x < 32; ++x) {
+      if (x > lim) v[x] = -INFINITY;
+    }
+  }
+}
+__device__ __forceinline__ float ca_most(const float (&v)[32], float top) {
+  float mx[4] = {top, v[0], v[1], v[2]};
+#pragma unroll
+  for (int x = 3; x < 31; x += 2) mx[(x / 2) & 3] = max3(mx[(x / 2) & 3], v[x], v[x + 1]);
+  return max3(max3(mx[0], mx[1], mx[2]), mx[3], v[31]);
+}
+// Their weights as bf16 pairs, and the weights' sums.
+__device__ __forceinline__ void ca_weigh(const float (&v)[32], uint64_t scale2, uint64_t shift2, uint64_t (&sums)[2],
+                                         uint32_t (&pk)[16]) {
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    const float2 z = unpair(fma2(pair(v[2 * x], v[2 * x + 1]), scale2, shift2));
+    const uint64_t p = (x & 7) >= 8 - kCaFmaGroups ? exp2_fma2(z.x, z.y) : pair(ex2_approx(z.x), ex2_approx(z.y));
+    sums[x & 1] = add2(sums[x & 1], p);
+    const float2 pf = unpair(p);
+    pk[x] = pack2(pf.x, pf.y);
+  }
+}
+
+// Joins the parts of a split tile, of ranges c0 .. c1 in that order. A thread
+// takes 8 columns of a pair at a time.
 template <int D>
-__device__ __forceinline__ void ca_join(const ChunkAttnArgs& a, int c0, int c1, int r, bf16* dst) {
-  for (int x0 = 0; x0 < D; x0 += 64) {
-    float m = kNegBig, l = 0.f;
-    float acc[64];
+__device__ __forceinline__ void ca_join(const ChunkAttnArgs& a, int c0, int c1, int pairs, bf16* out, int tid) {
+#pragma unroll 1
+  for (int item = tid; item < pairs * (D / 8); item += kCaRows) {
+    const int pair_r = item % pairs, x = item / pairs;
+    float m = kNegBig, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int k0 = c0; k0 <= c1; k0 += 4) {
+      float pm[4], pl[4];
+      float4 v[4][2];
 #pragma unroll
-    for (int x = 0; x < 64; ++x) acc[x] = 0.f;
-    for (int k = c0; k <= c1; ++k) {
-      const float* part = a.partials + static_cast<size_t>(2 * k + (k == c0 ? 1 : 0)) * ca_part_floats(D);
-      const float pm = __ldcg(part + r), pl = __ldcg(part + kCaRows + r);
-      const float nm = fmaxf(m, pm);
-      const float wa = ex2_approx(m - nm), wb = ex2_approx(pm - nm);
+      for (int i = 0; i < 4; ++i) {
+        const int k = min(k0 + i, c1);
+        const float* part = a.partials + static_cast<size_t>(2 * k + (k == c0 ? 1 : 0)) * ca_part_floats(D);
+        pm[i] = k0 + i <= c1 ? __ldcg(part + pair_r) : kNegBig;
+        pl[i] = __ldcg(part + kCaRows + pair_r);
+        const float4* p4 = reinterpret_cast<const float4*>(part + 2 * kCaRows) + pair_r;
+        v[i][0] = __ldcg(p4 + 2 * x * kCaRows);
+        v[i][1] = __ldcg(p4 + (2 * x + 1) * kCaRows);
+      }
+      const float nm = fmaxf(fmaxf(fmaxf(m, pm[0]), fmaxf(pm[1], pm[2])), pm[3]);
+      const float wa = ex2_approx(m - nm);
       m = nm;
-      l = l * wa + pl * wb;
-      const float4* p4 = reinterpret_cast<const float4*>(part + 2 * kCaRows) + (x0 / 4) * kCaRows + r;
+      l *= wa;
 #pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        const float4 v = __ldcg(p4 + x * kCaRows);
-        acc[4 * x] = fmaf(v.x, wb, acc[4 * x] * wa);
-        acc[4 * x + 1] = fmaf(v.y, wb, acc[4 * x + 1] * wa);
-        acc[4 * x + 2] = fmaf(v.z, wb, acc[4 * x + 2] * wa);
-        acc[4 * x + 3] = fmaf(v.w, wb, acc[4 * x + 3] * wa);
+      for (int y = 0; y < 8; ++y) acc[y] *= wa;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float wb = k0 + i <= c1 ? ex2_approx(pm[i] - nm) : 0.f;
+        l = fmaf(pl[i], wb, l);
+        acc[0] = fmaf(v[i][0].x, wb, acc[0]);
+        acc[1] = fmaf(v[i][0].y, wb, acc[1]);
+        acc[2] = fmaf(v[i][0].z, wb, acc[2]);
+        acc[3] = fmaf(v[i][0].w, wb, acc[3]);
+        acc[4] = fmaf(v[i][1].x, wb, acc[4]);
+        acc[5] = fmaf(v[i][1].y, wb, acc[5]);
+        acc[6] = fmaf(v[i][1].z, wb, acc[6]);
+        acc[7] = fmaf(v[i][1].w, wb, acc[7]);
       }
     }
     const float inv = ca_inverse(l);
-    uint4* d4 = reinterpret_cast<uint4*>(dst + x0);
-#pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      d4[x] = make_uint4(pack2(acc[8 * x] * inv, acc[8 * x + 1] * inv),
-                         pack2(acc[8 * x + 2] * inv, acc[8 * x + 3] * inv),
-                         pack2(acc[8 * x + 4] * inv, acc[8 * x + 5] * inv),
-                         pack2(acc[8 * x + 6] * inv, acc[8 * x + 7] * inv));
-    }
+    const int row = pair_r / a.group;
+    *reinterpret_cast<uint4*>(out + row * a.out_stride + (pair_r - row * a.group) * D + 8 * x) =
+        make_uint4(pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv), pack2(acc[4] * inv, acc[5] * inv),
+                   pack2(acc[6] * inv, acc[7] * inv));
   }
 }
 
@@ -438,6 +503,7 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
   struct Start {
     int part[kCaThreads / 32];
     int b, h, t, at;
+    int edge[2];
   };
   Start* st = reinterpret_cast<Start*>(ring);
   const int per_thread = (a.sequences + kCaThreads - 1) / kCaThreads;
@@ -465,22 +531,36 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
   const int ranges = min(static_cast<int>(gridDim.x), max(1, total / kCaMinRange));
   const int per = (total + ranges - 1) / ranges;
   const int c = blockIdx.x;
-  const bool some = static_cast<long long>(c) * per < total;
-  const int lo = some ? c * per : total, hi = min(total - lo, per) + lo;
-  if (lo >= before && lo < before + mine) {
-    int at = lo - before, b = b0;
-    for (int n = ca_seq<BLOCK>(a, b).units * a.kv_heads; at >= n; n = ca_seq<BLOCK>(a, b).units * a.kv_heads) {
-      at -= n;
-      ++b;
+  // Both ends, snapped; the thread whose requests hold an end finds it.
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+    const long long raw = static_cast<long long>(c + k) * per;
+    if (raw >= total) {
+      if (tid == 0) st->edge[k] = total;
+    } else if (raw >= before && raw < before + mine) {
+      int at = static_cast<int>(raw) - before, b = b0;
+      for (int n = ca_seq<BLOCK>(a, b).units * a.kv_heads; at >= n; n = ca_seq<BLOCK>(a, b).units * a.kv_heads) {
+        at -= n;
+        ++b;
+      }
+      CaWalk<BLOCK> e;
+      e.find(a, b, at);
+      const int shift = ca_snap(e.at, e.len + kCaTileCost);
+      const int edge = static_cast<int>(raw) + shift;
+      st->edge[k] = edge;
+      if (k == 0) {
+        e.at += shift;
+        if (shift > 0 && edge < total) e.advance(a);
+        st->b = e.b;
+        st->h = e.h;
+        st->t = e.t;
+        st->at = e.at;
+      }
     }
-    CaWalk<BLOCK> w;
-    w.find(a, b, at);
-    st->b = w.b;
-    st->h = w.h;
-    st->t = w.t;
-    st->at = w.at;
   }
   __syncthreads();
+  const int lo = st->edge[0], hi = st->edge[1];
+  const bool some = lo < hi;
   const int start_b = st->b, start_h = st->h, start_t = st->t, start_at = st->at;
   __syncthreads();  // the scratch becomes the ring
 
@@ -725,25 +805,27 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
   } else {
     // --- Softmax and epilogue: thread = pair r of the tile = TMEM lane --------
     const int r = tid;
-    const int qi = r / a.group, hl = r % a.group;
+    const int row_r = r / a.group, head_r = r - row_r * a.group;
     const uint32_t trow = tmem + (static_cast<uint32_t>(warp * 32) << 16);
     int g = 0;
     bool ok = true;
-    int parts = 0;        // parts stored so far
-    int done = lo;        // units before this segment
+    uint32_t parts = 0;  // parts stored so far
+    int done = lo;       // units before this segment
     do {
       const int cnt = w.count(), off = w.off();
       if (cnt == 0) {
         done += w.units();
         continue;
       }
-      const int row = (w.t << a.log2_qb) + qi;  // of the request
-      const bool live = qi < (1 << a.log2_qb) && row < w.q.n;
-      const long long head = static_cast<long long>(w.h * a.group + hl) * D;
+      const int row0 = w.t << a.log2_qb;  // of the request
+      const int pairs = min(1 << a.log2_qb, w.q.n - row0) * a.group;
+      const bool live = r < pairs;
+      const int row = row0 + row_r;
+      const long long head = static_cast<long long>(w.h * a.group + head_r) * D;
       // Every S of the tile before has landed (its last block's was waited for).
       {
         const uint4* src = reinterpret_cast<const uint4*>(a.q + (live ? (w.q.row0 + row) * a.q_stride + head : 0));
-#pragma unroll
+#pragma unroll 1
         for (int p = 0; p < G::PANELS; ++p) {
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
@@ -756,23 +838,14 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
       const int pos = live ? w.q.kv - w.q.n + row : -1;  // keys 0 .. pos
-      // The lowest position of the tile's rows: blocks that end below it need no mask.
-      const int low = w.q.kv - w.q.n + (w.t << a.log2_qb);
-      // A warp without a live pair (a request of a few rows fills the first
-      // warp at most) only keeps the barriers going.
+      const int low = w.q.kv - w.q.n + row0;  // blocks that end at or below it need no mask
+      // A warp without a live pair (a decoding request fills the first warp at
+      // most) only keeps the barriers going. Sharing such a tile's keys out over
+      // all four warps, with copies of Q in their lanes, shortened the chain by
+      // a fifth but was slower: 71 us instead of 65 for 64 requests of 1 - 5
+      // rows on 128 - 4096 keys (heads of 64), the extra warps in the way of
+      // the other CTAs' and four copies of O to join.
       const bool idle = !__any_sync(0xffffffffu, live);
-      auto most = [](const float (&v)[32], float top) {
-        float mx[4] = {max3(top, v[0], v[1]), max3(v[2], v[3], v[4]), max3(v[5], v[6], v[7]), v[8]};
-#pragma unroll
-        for (int x = 9; x < 25; x += 8) {
-#pragma unroll
-          for (int y = 0; y < 4; ++y) mx[y] = max3(mx[y], v[x + 2 * y], v[x + 2 * y + 1]);
-        }
-        mx[0] = max3(mx[0], v[25], v[26]);
-        mx[1] = max3(mx[1], v[27], v[28]);
-        mx[2] = max3(mx[2], v[29], v[30]);
-        return max3(max3(mx[0], mx[1], mx[2]), mx[3], v[31]);
-      };
       float m = kNegBig, l = 0.f;
       for (int j = 0; j < cnt; ++j, ++g) {
         // S of this block, and with it P V of the block before, have landed.
@@ -785,23 +858,12 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
         }
         const int lim = pos - (off + j) * BLOCK;  // keys of the block past it are masked
         const bool masked = (off + j + 1) * BLOCK - 1 > low;
-        float v[32];
-        auto fetch = [&](int c) {
-          tc_ld32(trow + 32 * c, v);
-          tc_wait_ld();
-          if (masked) {
-            asm volatile("" ::: "memory");  // a branch, not 32 predicated selects in every block
-#pragma unroll
-            for (int x = 0; x < 32; ++x) {
-              if (32 * c + x > lim) v[x] = -INFINITY;
-            }
-          }
-        };
         float top = -INFINITY;
 #pragma unroll 1
-        for (int c = 0; c < BLOCK / 32; ++c) {
-          fetch(c);
-          top = most(v, top);
+        for (int c = 0; c < BLOCK; c += 32) {
+          float v[32];
+          ca_fetch(trow + c, v, masked, lim - c);
+          top = ca_most(v, top);
         }
         top *= a.scale_log2;
         const bool grow = top > m + 8.0f;  // false for a row with no key yet: m stays at its lowest
@@ -825,18 +887,12 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
         uint64_t sums[2] = {0, 0};
         const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), shift2 = pair(-m, -m);
 #pragma unroll 1
-        for (int c = 0; c < BLOCK / 32; ++c) {
-          fetch(c);
+        for (int c = 0; c < BLOCK; c += 32) {
+          float v[32];
           uint32_t pk[16];
-#pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const float2 z = unpair(fma2(pair(v[2 * x], v[2 * x + 1]), scale2, shift2));
-            const uint64_t p = (x & 7) >= 8 - kCaFmaGroups ? exp2_fma2(z.x, z.y) : pair(ex2_approx(z.x), ex2_approx(z.y));
-            sums[x & 1] = add2(sums[x & 1], p);
-            const float2 pf = unpair(p);
-            pk[x] = pack2(pf.x, pf.y);
-          }
-          tc_st16u(trow + 16 * c, pk);  // over scores that have been read
+          ca_fetch(trow + c, v, masked, lim - c);
+          ca_weigh(v, scale2, shift2, sums, pk);
+          tc_st16u(trow + c / 2, pk);  // over scores that have been read
         }
         const float2 sum = unpair(add2(sums[0], sums[1]));
         l += sum.x + sum.y;
@@ -849,10 +905,10 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
       ok = __all_sync(0xffffffffu, ca_wait(pv_done, (g - 1) & 1, a.status, kStatusTimeoutFull));
       if (!ok) break;
       tc_fence_after();
-      bf16* dst = a.out + (live ? (w.q.row0 + row) * a.out_stride + head : 0);
       if (cnt == w.len) {
         const float inv = ca_inverse(l);
-#pragma unroll
+        bf16* dst = a.out + (live ? (w.q.row0 + row) * a.out_stride + head : 0);
+#pragma unroll 1
         for (int x = 0; x < D; x += 16) {
           float o[16];
           tc_ld16(trow + G::O_COL + x, o);
@@ -868,36 +924,36 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
           }
         }
       } else {
-        // A part: columns of four as [column / 4][pair], so neighbouring
+        // A part: columns of four as [column / 4][lane], so neighbouring
         // threads' 16 bytes are neighbours.
-        const int tile0 = done - w.at + kCaTileCost;  // unit of the tile's first block
         float* part = a.partials + static_cast<size_t>(2 * c + (off > 0 ? 0 : 1)) * ca_part_floats(D);
         if (live) {
           part[r] = m;
           part[kCaRows + r] = l;
         }
-#pragma unroll
+        float4* p4 = reinterpret_cast<float4*>(part + 2 * kCaRows) + r;
+#pragma unroll 1
         for (int x = 0; x < D; x += 16) {
           float o[16];
           tc_ld16(trow + G::O_COL + x, o);
           tc_wait_ld();
           if (live) {
-            float4* p4 = reinterpret_cast<float4*>(part + 2 * kCaRows);
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-              p4[(x / 4 + y) * kCaRows + r] = make_float4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]);
+              p4[(x / 4 + y) * kCaRows] = make_float4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]);
             }
           }
         }
-        const int c0 = tile0 / per, c1 = (tile0 + w.len - 1) / per;  // the ranges of its first and last block
-        __threadfence();
+        // The ranges of the tile's first and last block.
+        const int tile0 = done - w.at, units = w.len + kCaTileCost;
+        const int c0 = ca_owner(tile0 + kCaTileCost, tile0, units, per), c1 = ca_owner(tile0 + units - 1, tile0, units, per);
         __syncwarp();
         if (lane == 0) mbar_arrive(stored);
         ok = __all_sync(0xffffffffu, ca_wait(stored, parts & 1, a.status, kStatusTimeoutFull));
         if (!ok) break;
         if (tid == 0) {
-          const unsigned n = atomicAdd(&a.counters[c0], 1u) + 1u;
-          const bool last = n == static_cast<unsigned>(c1 - c0 + 1);
+          __threadfence();  // what the CTA's threads stored before they met, too
+          const bool last = atomicAdd(&a.counters[c0], 1u) == static_cast<unsigned>(c1 - c0);
           if (last) a.counters[c0] = 0u;
           *last_s = last;
           __threadfence();
@@ -906,7 +962,9 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
         ok = __all_sync(0xffffffffu, ca_wait(counted, parts & 1, a.status, kStatusTimeoutFull));
         if (!ok) break;
         ++parts;
-        if (*last_s && live) ca_join<D>(a, c0, c1, r, dst);
+        if (*last_s) {
+          ca_join<D>(a, c0, c1, pairs, a.out + (w.q.row0 + row0) * a.out_stride + w.h * a.group * D, tid);
+        }
       }
       tc_fence_before();  // O and S were read: the next tile's MMAs may write them
       done += w.units();
