@@ -37,6 +37,24 @@ int check_view(const char* what, const lcr_kv_view* v, int pool_pages) {
   return LCR_OK;
 }
 
+// A launch in clusters of `ctas` CTAs along x.
+template <class Args>
+int launch_cluster(void (*kernel)(Args), int grid, int ctas, int threads, cudaStream_t s, const Args& args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args);
+  return e == cudaSuccess ? LCR_OK : fail(LCR_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
+}
+
 // CTAs of the chunk attention on the current device; the workspace holds a
 // status word, a counter for each, and two parts for each.
 int attention_ctas(int head_dim) {
@@ -99,7 +117,7 @@ extern "C" int lcr_plan_step(int32_t* block_tables, int max_pages, const int32_t
                     row_starts,   kv_lengths, positions, slots,      row_sequence};
   const size_t smem = sizeof(int32_t) * 4 * static_cast<size_t>(sequences);
   LCRB_CUDA(cudaFuncSetAttribute(step_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  return launch_kernel(step_plan_kernel, dim3(1), dim3(kPlanThreads), smem, cs(stream), false, a);
+  return launch_kernel(step_plan_kernel, dim3(kPlanCtas), dim3(kPlanThreads), smem, cs(stream), false, a);
 }
 
 extern "C" int lcr_qk_norm_rope_kv(void* q_out, int64_t q_stride, const lcr_kv_view* view, int pool_pages,
@@ -240,9 +258,16 @@ extern "C" int lcr_token_probs(float* probs, int64_t probs_stride, const float* 
   LCRB_REQUIRE(probs_stride >= vocab && logits_stride >= vocab, LCR_ERR_INVALID,
                "token_probs: row strides %lld and %lld of %d ids", static_cast<long long>(probs_stride),
                static_cast<long long>(logits_stride), vocab);
-  TokenProbsArgs a = {probs, probs_stride, logits, logits_stride, rows, vocab, temperature, row_sequence};
-  return launch_kernel(token_probs_kernel, dim3(static_cast<unsigned>(rows)), dim3(kProbsThreads), 0, cs(stream), false,
-                       a);
+  TokenProbsArgs a = {probs, probs_stride, logits, logits_stride, rows, vocab, temperature, row_sequence, 0};
+  // CTAs for a row: enough to keep it in registers, and for few rows as many as
+  // fill the GPU (one row of 128256 ids: 8 CTAs).
+  int ctas = 1;
+  while (ctas < kProbsMaxCtas && (vocab > ctas * kProbsSlice || (rows * ctas < 256 && vocab > ctas * 2048))) ctas *= 2;
+  LCRB_REQUIRE(rows <= INT32_MAX / ctas, LCR_ERR_SHAPE, "token_probs: %d rows", rows);
+  a.slice = ((vocab + ctas - 1) / ctas + 3) / 4 * 4;
+  const bool vec = aligned16(probs) && aligned16(logits) && probs_stride % 4 == 0 && logits_stride % 4 == 0;
+  return launch_cluster(vec ? token_probs_kernel<true> : token_probs_kernel<false>, rows * ctas, ctas, kProbsThreads,
+                        cs(stream), a);
 }
 
 extern "C" int lcr_verify_drafts(int32_t* tokens, int32_t* accepted, const float* target_probs, int64_t target_stride,
@@ -257,6 +282,7 @@ extern "C" int lcr_verify_drafts(int32_t* tokens, int32_t* accepted, const float
                static_cast<long long>(target_stride), vocab);
   VerifyArgs a = {tokens,      accepted, target_probs, target_stride, target_starts, drafts, draft_counts,
                   draft_probs, uniforms, sequences,    max_drafts,    vocab};
-  return launch_kernel(verify_drafts_kernel, dim3(static_cast<unsigned>(sequences)), dim3(kVerifyThreads), 0,
+  LCRB_REQUIRE(sequences <= INT32_MAX / kVerifyCtas, LCR_ERR_SHAPE, "verify_drafts: %d requests", sequences);
+  return launch_kernel(verify_drafts_kernel, dim3(static_cast<unsigned>(sequences) * kVerifyCtas), dim3(kVerifyThreads), 0,
                        cs(stream), false, a);
 }

@@ -43,78 +43,100 @@ __device__ __forceinline__ float2 rope_pair(int position, float inv_freq) {
   return make_float2(fmaf(-err, s, c), fmaf(err, c, s));
 }
 
-constexpr int kQkThreads = 256;
+// Two bf16 in one conversion.
+__device__ __forceinline__ uint32_t qk_pack(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+constexpr int kQkThreads = 192;
+constexpr int kQkItems = 2;  // a thread's pieces in flight
 
 // One CTA per row. A group of D/16 lanes owns a head: each lane holds 8
 // elements of its lower and 8 of its upper half, so the rotation needs no
-// exchange and the sum of squares log2(D/16) shuffles.
+// exchange and the sum of squares log2(D/16) shuffles. HBM bound: a thread's
+// loads (64 bytes) are issued before the row's angles are formed, and ten CTAs
+// share an SM, so that one row's latencies hide under the others' transfers.
 template <int D>
 __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkNormRopeArgs a) {
   constexpr int HALF = D / 2;
   constexpr int LANES = D / 16;
   __shared__ float2 cs[HALF];
   const int r = blockIdx.x, tid = threadIdx.x;
-  for (int i = tid; i < HALF; i += kQkThreads) cs[i] = rope_pair(a.positions[r], a.inv_freq[i]);
-  const int slot = a.slots[r];
-  const bool cached = slot >= 0 && slot / a.page_size < a.pool_pages;
-  const long long at = cached ? static_cast<long long>(slot / a.page_size) * a.page_stride +
-                                    static_cast<long long>(slot % a.page_size) * D
-                              : 0;
-  __syncthreads();
   const bf16* row = a.qkv + r * a.qkv_stride;
   const int items = (a.heads + 2 * a.kv_heads) * LANES;
   const int piece = (tid % LANES) * 8;
+  uint4 rl[kQkItems], rh[kQkItems];
+  auto load = [&](int first) {
+#pragma unroll
+    for (int k = 0; k < kQkItems; ++k) {
+      const int it = first + k * kQkThreads;
+      const bf16* src = row + (it < items ? it / LANES : 0) * D + piece;
+      rl[k] = ldg16(src);
+      rh[k] = ldg16(src + HALF);
+    }
+  };
+  load(tid);
+  const int slot = a.slots[r];
+  const int page = slot / a.page_size;
+  const bool cached = slot >= 0 && page < a.pool_pages;
+  const long long at = cached ? page * a.page_stride + static_cast<long long>(slot - page * a.page_size) * D : 0;
+  if (tid < HALF) cs[tid] = rope_pair(a.positions[r], a.inv_freq[tid]);
+  __syncthreads();
   // Every lane takes part in the shuffles: the loop count is uniform.
-  for (int it = tid; it - tid < items; it += kQkThreads) {
-    const bool live = it < items;
-    const int h = live ? it / LANES : 0;
-    const bf16* src = row + h * D + piece;
-    const uint4 rl = live ? ldg16(src) : make_uint4(0u, 0u, 0u, 0u);
-    const uint4 rh = live ? ldg16(src + HALF) : make_uint4(0u, 0u, 0u, 0u);
-    float lo[8], hi[8];
-    unpack8(rl, lo);
-    unpack8(rh, hi);
-    const bool is_v = h >= a.heads + a.kv_heads, is_q = h < a.heads;
-    const bf16* gain = is_q ? a.q_gain : a.k_gain;
-    float ss = 0.f;
+  for (int first = tid; first - tid < items; first += kQkItems * kQkThreads) {
+    if (first != tid) load(first);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
+    for (int k = 0; k < kQkItems; ++k) {
+      const int it = first + k * kQkThreads;
+      const bool live = it < items;
+      const int h = live ? it / LANES : 0;
+      float lo[8], hi[8];
+      unpack8(rl[k], lo);
+      unpack8(rh[k], hi);
+      const bool is_v = h >= a.heads + a.kv_heads, is_q = h < a.heads;
+      const bf16* gain = is_q ? a.q_gain : a.k_gain;
+      float ss = 0.f;
 #pragma unroll
-    for (int off = LANES / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-    if (!live) continue;
-    uint4 wl = rl, wh = rh;
-    if (!is_v) {
-      if (gain != nullptr) {
-        const float scale = rsqrtf(ss * (1.0f / D) + a.eps);
-        float gl[8], gh[8];
-        unpack8(ldg16(gain + piece), gl);
-        unpack8(ldg16(gain + HALF + piece), gh);
+      for (int e = 0; e < 8; ++e) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
+#pragma unroll
+      for (int off = LANES / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+      if (!live) continue;
+      uint4 wl = rl[k], wh = rh[k];
+      if (!is_v) {
+        if (gain != nullptr) {
+          const float scale = rsqrtf(ss * (1.0f / D) + a.eps);
+          float gl[8], gh[8];
+          unpack8(ldg16(gain + piece), gl);
+          unpack8(ldg16(gain + HALF + piece), gh);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            lo[e] = lo[e] * scale * gl[e];
+            hi[e] = hi[e] * scale * gh[e];
+          }
+        }
+        float ol[8], oh[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          lo[e] = lo[e] * scale * gl[e];
-          hi[e] = hi[e] * scale * gh[e];
+          const float2 t = cs[piece + e];
+          ol[e] = lo[e] * t.x - hi[e] * t.y;
+          oh[e] = hi[e] * t.x + lo[e] * t.y;
         }
+        wl = make_uint4(qk_pack(ol[0], ol[1]), qk_pack(ol[2], ol[3]), qk_pack(ol[4], ol[5]), qk_pack(ol[6], ol[7]));
+        wh = make_uint4(qk_pack(oh[0], oh[1]), qk_pack(oh[2], oh[3]), qk_pack(oh[4], oh[5]), qk_pack(oh[6], oh[7]));
       }
-      float ol[8], oh[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float2 t = cs[piece + e];
-        ol[e] = lo[e] * t.x - hi[e] * t.y;
-        oh[e] = hi[e] * t.x + lo[e] * t.y;
+      bf16* dst;
+      if (is_q) {
+        dst = a.q_out + r * a.q_stride + h * D + piece;
+      } else {
+        if (!cached) continue;
+        const int kvh = is_v ? h - a.heads - a.kv_heads : h - a.heads;
+        dst = (is_v ? a.values : a.keys) + at + kvh * a.head_stride + piece;
       }
-      wl = make_uint4(pack_bf2(ol[0], ol[1]), pack_bf2(ol[2], ol[3]), pack_bf2(ol[4], ol[5]), pack_bf2(ol[6], ol[7]));
-      wh = make_uint4(pack_bf2(oh[0], oh[1]), pack_bf2(oh[2], oh[3]), pack_bf2(oh[4], oh[5]), pack_bf2(oh[6], oh[7]));
+      *reinterpret_cast<uint4*>(dst) = wl;
+      *reinterpret_cast<uint4*>(dst + HALF) = wh;
     }
-    bf16* dst;
-    if (is_q) {
-      dst = a.q_out + r * a.q_stride + h * D + piece;
-    } else {
-      if (!cached) continue;
-      const int kvh = is_v ? h - a.heads - a.kv_heads : h - a.heads;
-      dst = (is_v ? a.values : a.keys) + at + kvh * a.head_stride + piece;
-    }
-    *reinterpret_cast<uint4*>(dst) = wl;
-    *reinterpret_cast<uint4*>(dst + HALF) = wh;
   }
 }
 

@@ -9,11 +9,14 @@
 // inclusive prefix of needs is at most F.
 #pragma once
 
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 
 namespace lcrb {
 
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanCtas = 8;  // one cluster
 
 struct StepPlanArgs {
   int32_t* tables;
@@ -72,8 +75,14 @@ __device__ __forceinline__ int plan_add_rows(int x, int y, int most) {
   return s < static_cast<uint32_t>(most) ? static_cast<int>(s) : most;
 }
 
-// One CTA: scan, push, hand out, rows, with a block barrier between.
-__global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const StepPlanArgs a) {
+// One cluster of eight CTAs. Every CTA scans all requests (a few loads and
+// shuffles; cheaper than passing the prefixes on), then they share the pages
+// and the rows; cluster barriers stand between pushing pages, handing them out
+// and reading the tables back, so held and free_count may be updated in place.
+// A step of a few rows is bound by latency -- launch, the lengths' load, two
+// block barriers, a cluster barrier, the table's load -- and a large one by the
+// rows' stores, four rows a thread.
+__global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) step_plan_kernel(const StepPlanArgs a) {
   extern __shared__ int32_t plan_smem[];
   int32_t* row_end = plan_smem;            // inclusive prefixes per request
   int32_t* need_end = row_end + a.sequences;
@@ -81,8 +90,12 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const StepPlanA
   int32_t* base = back_end + a.sequences;  // pages held before this step's
   __shared__ int part[3][kPlanThreads / 32];
   __shared__ int used_s;
+  const auto cluster = cooperative_groups::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int me = static_cast<int>(cluster.block_rank()) * kPlanThreads + tid;
+  constexpr int kAll = kPlanCtas * kPlanThreads;
   const int B = a.sequences;
+  const int free0 = min(max(0, *a.free_count), a.pool_pages);
 
   // Thread t scans a contiguous share of the requests.
   const int per = (B + kPlanThreads - 1) / kPlanThreads;
@@ -98,17 +111,20 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const StepPlanA
     back_end[b] = back;
     base[b] = r.held;
   }
-  int irows = rows, ineed = need, iback = back;
+  auto scan = [&](int& x, int& y, int& z) {  // inclusive, over a warp
 #pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, irows, off), y = __shfl_up_sync(0xffffffffu, ineed, off),
-              z = __shfl_up_sync(0xffffffffu, iback, off);
-    if (lane >= off) {
-      irows = plan_add_rows(irows, x, a.max_rows);
-      ineed += y;
-      iback += z;
+    for (int off = 1; off < 32; off <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, x, off), v = __shfl_up_sync(0xffffffffu, y, off),
+                t = __shfl_up_sync(0xffffffffu, z, off);
+      if (lane >= off) {
+        x = plan_add_rows(x, u, a.max_rows);
+        y += v;
+        z += t;
+      }
     }
-  }
+  };
+  int irows = rows, ineed = need, iback = back;
+  scan(irows, ineed, iback);
   if (lane == 31) {
     part[0][warp] = irows;
     part[1][warp] = ineed;
@@ -116,12 +132,14 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const StepPlanA
   }
   if (tid == 0) used_s = 0;
   __syncthreads();
-  int prow = 0, pneed = 0, pback = 0;  // exclusive prefixes of this thread
-  for (int w = 0; w < warp; ++w) {
-    prow = plan_add_rows(prow, part[0][w], a.max_rows);
-    pneed += part[1][w];
-    pback += part[2][w];
-  }
+  // The warps' totals, scanned by every warp; then this thread's exclusive
+  // prefixes.
+  int wrows = part[0][lane], wneed = part[1][lane], wback = part[2][lane];
+  scan(wrows, wneed, wback);
+  const int total_back = __shfl_sync(0xffffffffu, wback, 31);
+  int prow = __shfl_sync(0xffffffffu, wrows, max(0, warp - 1)), pneed = __shfl_sync(0xffffffffu, wneed, max(0, warp - 1)),
+      pback = __shfl_sync(0xffffffffu, wback, max(0, warp - 1));
+  if (warp == 0) prow = pneed = pback = 0;
   {
     const int x = __shfl_up_sync(0xffffffffu, irows, 1), y = __shfl_up_sync(0xffffffffu, ineed, 1),
               z = __shfl_up_sync(0xffffffffu, iback, 1);
@@ -131,9 +149,6 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const StepPlanA
       pback += z;
     }
   }
-  int total_back = 0;
-  for (int w = 0; w < kPlanThreads / 32; ++w) total_back += part[2][w];
-  const int free0 = min(max(0, *a.free_count), a.pool_pages);
   const int height = min(free0 + total_back, a.pool_pages);
   int used = 0;
   for (int b = b0; b < b1; ++b) {
@@ -150,51 +165,88 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const StepPlanA
   const int pushed = height - free0;
 
   // Pages given back, on top of the free ones.
-  for (int k = tid; k < pushed; k += kPlanThreads) {
-    const int b = plan_owner(back_end, B, k);
-    const int first = b > 0 ? back_end[b - 1] : 0;
-    a.free_pages[free0 + k] = a.tables[static_cast<size_t>(b) * a.max_pages + (k - first)];
+  if (pushed > 0) {
+    for (int k = me; k < pushed; k += kAll) {
+      const int b = plan_owner(back_end, B, k);
+      const int first = b > 0 ? back_end[b - 1] : 0;
+      a.free_pages[free0 + k] = a.tables[static_cast<size_t>(b) * a.max_pages + (k - first)];
+    }
+    cluster.sync();
   }
-  __syncthreads();
   // Pages handed out, from the top.
-  for (int k = tid; k < used; k += kPlanThreads) {
+  for (int k = me; k < used; k += kAll) {
     const int b = plan_owner(need_end, B, k);
     const int first = b > 0 ? need_end[b - 1] : 0;
-    a.tables[static_cast<size_t>(b) * a.max_pages + base[b] + (k - first)] = a.free_pages[height - 1 - k];
+    a.tables[static_cast<size_t>(b) * a.max_pages + base[b] + (k - first)] = __ldcg(a.free_pages + height - 1 - k);
   }
-  __syncthreads();
-  // Per request (held may be held_out, free_count free_count_out: every
-  // thread has read them).
-  for (int b = b0; b < b1; ++b) {
-    const int c = max(0, a.cached[b]), n = max(0, a.new_tokens[b]);
+  cluster.sync();
+  auto granted = [&](int b, int c, int n) {
     const long long want = (static_cast<long long>(c) + n + a.page_size - 1) / a.page_size;
     const int nb = need_end[b] - (b > 0 ? need_end[b - 1] : 0);
-    const bool granted = want <= a.max_pages && (nb == 0 || need_end[b] <= height);
-    a.row_starts[b] = b > 0 ? row_end[b - 1] : 0;
-    a.held_out[b] = base[b] + (granted ? nb : 0);
-    a.kv_lengths[b] = granted ? c + n : 0;
-  }
-  if (tid == 0) {
-    a.row_starts[B] = row_end[B - 1];
-    *a.free_count_out = height - used;
-  }
-  const int total = row_end[B - 1];
-  for (int r = tid; r < total; r += kPlanThreads) {
-    const int b = plan_owner(row_end, B, r);
-    const int i = r - (b > 0 ? row_end[b - 1] : 0);
-    const int c = max(0, a.cached[b]), n = max(0, a.new_tokens[b]);
-    const long long want = (static_cast<long long>(c) + n + a.page_size - 1) / a.page_size;
-    const int nb = need_end[b] - (b > 0 ? need_end[b - 1] : 0);
-    const bool granted = want <= a.max_pages && (nb == 0 || need_end[b] <= height);
-    const int pos = c + i;
-    int slot = -1;
-    if (granted) {
-      const int page = a.tables[static_cast<size_t>(b) * a.max_pages + pos / a.page_size];
-      if (page >= 0 && page < a.pool_pages) slot = page * a.page_size + pos % a.page_size;
+    return want <= a.max_pages && (nb == 0 || need_end[b] <= height);
+  };
+  // Per request, by one CTA (held may be held_out, free_count free_count_out:
+  // every thread of the cluster has read them).
+  if (cluster.block_rank() == 0) {
+    for (int b = b0; b < b1; ++b) {
+      const int c = max(0, a.cached[b]), n = max(0, a.new_tokens[b]);
+      const bool got = granted(b, c, n);
+      a.row_starts[b] = b > 0 ? row_end[b - 1] : 0;
+      a.held_out[b] = base[b] + (got ? need_end[b] - (b > 0 ? need_end[b - 1] : 0) : 0);
+      a.kv_lengths[b] = got ? c + n : 0;
     }
-    a.positions[r] = pos;
-    a.slots[r] = slot;
-    a.row_sequence[r] = b;
+    if (tid == 0) {
+      a.row_starts[B] = row_end[B - 1];
+      *a.free_count_out = height - used;
+    }
+  }
+  // Four neighbouring rows a thread: one search, and 16-byte stores.
+  const int total = row_end[B - 1];
+  const bool wide = ((reinterpret_cast<uintptr_t>(a.positions) | reinterpret_cast<uintptr_t>(a.slots) |
+                      reinterpret_cast<uintptr_t>(a.row_sequence)) & 15u) == 0;
+  for (int r0 = 4 * me; r0 < total; r0 += 4 * kAll) {
+    int b = plan_owner(row_end, B, r0);
+    int begin = b > 0 ? row_end[b - 1] : 0, end = row_end[b];
+    int c = max(0, a.cached[b]), n = max(0, a.new_tokens[b]);
+    bool got = granted(b, c, n);
+    int pos[4], slot[4], seq[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = r0 + e;
+      if (r < total) {
+        if (r >= end) {
+          do {
+            begin = end;
+            end = row_end[++b];
+          } while (r >= end);
+          c = max(0, a.cached[b]);
+          n = max(0, a.new_tokens[b]);
+          got = granted(b, c, n);
+        }
+        pos[e] = c + (r - begin);
+        slot[e] = -1;
+        seq[e] = b;
+        if (got) {
+          const int q = pos[e] / a.page_size;
+          const int page = __ldcg(a.tables + static_cast<size_t>(b) * a.max_pages + q);
+          if (page >= 0 && page < a.pool_pages) slot[e] = page * a.page_size + pos[e] - q * a.page_size;
+        }
+      }
+    }
+    if (wide && r0 + 4 <= total) {
+      *reinterpret_cast<int4*>(a.positions + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+      *reinterpret_cast<int4*>(a.slots + r0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+      *reinterpret_cast<int4*>(a.row_sequence + r0) = make_int4(seq[0], seq[1], seq[2], seq[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (r0 + e < total) {
+          a.positions[r0 + e] = pos[e];
+          a.slots[r0 + e] = slot[e];
+          a.row_sequence[r0 + e] = seq[e];
+        }
+      }
+    }
   }
 }
 
