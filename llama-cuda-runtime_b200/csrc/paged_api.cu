@@ -37,6 +37,17 @@ int check_view(const char* what, const lcr_kv_view* v, int pool_pages) {
   return LCR_OK;
 }
 
+// Of the current device.
+int multiprocessors() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 148;
+  }
+  return sms;
+}
+
 // A launch in clusters of `ctas` CTAs along x.
 template <class Args>
 int launch_cluster(void (*kernel)(Args), int grid, int ctas, int threads, cudaStream_t s, const Args& args) {
@@ -57,15 +68,7 @@ int launch_cluster(void (*kernel)(Args), int grid, int ctas, int threads, cudaSt
 
 // CTAs of the chunk attention on the current device; the workspace holds a
 // status word, a counter for each, and two parts for each.
-int attention_ctas(int head_dim) {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-    cudaGetLastError();
-    sms = 148;
-  }
-  return (head_dim == 64 ? CaGeom<64>::CTAS : CaGeom<128>::CTAS) * sms;
-}
+int attention_ctas(int head_dim) { return (head_dim == 64 ? CaGeom<64>::CTAS : CaGeom<128>::CTAS) * multiprocessors(); }
 size_t attention_header(size_t ctas) { return 256 + (ctas * sizeof(unsigned) + 255) / 256 * 256; }
 
 template <int D, bool TMA>
@@ -156,7 +159,8 @@ extern "C" int lcr_qk_norm_rope_kv(void* q_out, int64_t q_stride, const lcr_kv_v
   a.positions = positions;
   a.slots = slots;
   auto kernel = view->head_dim == 64 ? qk_norm_rope_kernel<64> : qk_norm_rope_kernel<128>;
-  return launch_kernel(kernel, dim3(static_cast<unsigned>(rows)), dim3(kQkThreads), 0, cs(stream), false, a);
+  return launch_kernel(kernel, dim3(static_cast<unsigned>(std::min(rows, kQkCtas * multiprocessors()))), dim3(kQkThreads), 0,
+                       cs(stream), false, a);
 }
 
 extern "C" size_t lcr_chunk_attention_scratch_bytes(int num_heads, int head_dim) {
@@ -282,7 +286,8 @@ extern "C" int lcr_verify_drafts(int32_t* tokens, int32_t* accepted, const float
                static_cast<long long>(target_stride), vocab);
   VerifyArgs a = {tokens,      accepted, target_probs, target_stride, target_starts, drafts, draft_counts,
                   draft_probs, uniforms, sequences,    max_drafts,    vocab};
-  LCRB_REQUIRE(sequences <= INT32_MAX / kVerifyCtas, LCR_ERR_SHAPE, "verify_drafts: %d requests", sequences);
-  return launch_kernel(verify_drafts_kernel, dim3(static_cast<unsigned>(sequences) * kVerifyCtas), dim3(kVerifyThreads), 0,
-                       cs(stream), false, a);
+  // CTAs for a request: as many as run at once (two on an SM) for all of them.
+  int ctas = 1;
+  while (ctas < kVerifyMaxCtas && static_cast<long long>(sequences) * ctas * 2 <= 296) ctas *= 2;
+  return launch_cluster(verify_drafts_kernel, sequences * ctas, ctas, kVerifyThreads, cs(stream), a);
 }

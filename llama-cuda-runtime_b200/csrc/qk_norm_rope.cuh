@@ -51,50 +51,60 @@ __device__ __forceinline__ uint32_t qk_pack(float lo, float hi) {
 }
 
 constexpr int kQkThreads = 192;
-constexpr int kQkItems = 2;  // a thread's pieces in flight
+constexpr int kQkAhead = 2;  // pieces of a row that a thread holds ahead
+constexpr int kQkCtas = 4;   // per SM
 
-// One CTA per row. A group of D/16 lanes owns a head: each lane holds 8
-// elements of its lower and 8 of its upper half, so the rotation needs no
-// exchange and the sum of squares log2(D/16) shuffles. HBM bound: a thread's
-// loads (64 bytes) are issued before the row's angles are formed, and ten CTAs
-// share an SM, so that one row's latencies hide under the others' transfers.
+// A group of D/16 lanes owns a head: each lane holds 8 elements of its lower
+// and 8 of its upper half (a piece), so the rotation needs no exchange and the
+// sum of squares log2(D/16) shuffles. HBM bound: every CTA walks over rows and
+// loads the next row's pieces (64 bytes a thread), position and slot before it
+// works on the present one, so that loads are always in flight; the angles'
+// pairs, by head_dim / 2 threads, are double-buffered, with one barrier a row.
 template <int D>
-__global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkNormRopeArgs a) {
+__global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kernel(const QkNormRopeArgs a) {
   constexpr int HALF = D / 2;
   constexpr int LANES = D / 16;
-  __shared__ float2 cs[HALF];
-  const int r = blockIdx.x, tid = threadIdx.x;
-  const bf16* row = a.qkv + r * a.qkv_stride;
+  __shared__ float2 cs[2][HALF];
+  const int tid = threadIdx.x;
   const int items = (a.heads + 2 * a.kv_heads) * LANES;
   const int piece = (tid % LANES) * 8;
-  uint4 rl[kQkItems], rh[kQkItems];
-  auto load = [&](int first) {
-#pragma unroll
-    for (int k = 0; k < kQkItems; ++k) {
-      const int it = first + k * kQkThreads;
-      const bf16* src = row + (it < items ? it / LANES : 0) * D + piece;
-      rl[k] = ldg16(src);
-      rh[k] = ldg16(src + HALF);
-    }
+  const float freq = tid < HALF ? a.inv_freq[tid] : 0.f;
+  uint4 next[kQkAhead][2];
+  int next_pos, next_slot;
+  auto fetch = [&](int r, int it, uint4 (&v)[2]) {
+    const bf16* src = a.qkv + r * a.qkv_stride + (it < items ? it / LANES : 0) * D + piece;
+    v[0] = ldg16(src);
+    v[1] = ldg16(src + HALF);
   };
-  load(tid);
-  const int slot = a.slots[r];
-  const int page = slot / a.page_size;
-  const bool cached = slot >= 0 && page < a.pool_pages;
-  const long long at = cached ? page * a.page_stride + static_cast<long long>(slot - page * a.page_size) * D : 0;
-  if (tid < HALF) cs[tid] = rope_pair(a.positions[r], a.inv_freq[tid]);
-  __syncthreads();
-  // Every lane takes part in the shuffles: the loop count is uniform.
-  for (int first = tid; first - tid < items; first += kQkItems * kQkThreads) {
-    if (first != tid) load(first);
+  auto ahead = [&](int r) {
 #pragma unroll
-    for (int k = 0; k < kQkItems; ++k) {
-      const int it = first + k * kQkThreads;
+    for (int k = 0; k < kQkAhead; ++k) fetch(r, tid + k * kQkThreads, next[k]);
+    next_pos = a.positions[r];
+    next_slot = a.slots[r];
+  };
+  ahead(blockIdx.x);
+  int buf = 0;
+  for (int r = blockIdx.x; r < a.rows; r += gridDim.x, buf ^= 1) {
+    uint4 now[kQkAhead][2];
+#pragma unroll
+    for (int k = 0; k < kQkAhead; ++k) {
+      now[k][0] = next[k][0];
+      now[k][1] = next[k][1];
+    }
+    const int slot = next_slot;
+    if (tid < HALF) cs[buf][tid] = rope_pair(next_pos, freq);
+    if (r + static_cast<int>(gridDim.x) < a.rows) ahead(r + gridDim.x);
+    const int page = slot / a.page_size;
+    const bool cached = slot >= 0 && page < a.pool_pages;
+    const long long at = cached ? page * a.page_stride + static_cast<long long>(slot - page * a.page_size) * D : 0;
+    __syncthreads();
+    // (Every lane of a group takes part in the shuffles: a group is live or not.)
+    auto work = [&](int it, const uint4 (&v)[2]) {
       const bool live = it < items;
       const int h = live ? it / LANES : 0;
       float lo[8], hi[8];
-      unpack8(rl[k], lo);
-      unpack8(rh[k], hi);
+      unpack8(v[0], lo);
+      unpack8(v[1], hi);
       const bool is_v = h >= a.heads + a.kv_heads, is_q = h < a.heads;
       const bf16* gain = is_q ? a.q_gain : a.k_gain;
       float ss = 0.f;
@@ -102,40 +112,43 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkNormRo
       for (int e = 0; e < 8; ++e) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
 #pragma unroll
       for (int off = LANES / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-      if (!live) continue;
-      uint4 wl = rl[k], wh = rh[k];
+      uint4 wl = v[0], wh = v[1];
       if (!is_v) {
         if (gain != nullptr) {
           const float scale = rsqrtf(ss * (1.0f / D) + a.eps);
-          float gl[8], gh[8];
-          unpack8(ldg16(gain + piece), gl);
-          unpack8(ldg16(gain + HALF + piece), gh);
+          float g[8];
+          unpack8(ldg16(gain + piece), g);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            lo[e] = lo[e] * scale * gl[e];
-            hi[e] = hi[e] * scale * gh[e];
-          }
+          for (int e = 0; e < 8; ++e) lo[e] = lo[e] * scale * g[e];
+          unpack8(ldg16(gain + HALF + piece), g);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) hi[e] = hi[e] * scale * g[e];
         }
-        float ol[8], oh[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float2 t = cs[piece + e];
-          ol[e] = lo[e] * t.x - hi[e] * t.y;
-          oh[e] = hi[e] * t.x + lo[e] * t.y;
+          const float2 t = cs[buf][piece + e];
+          const float x = lo[e], y = hi[e];
+          lo[e] = x * t.x - y * t.y;
+          hi[e] = y * t.x + x * t.y;
         }
-        wl = make_uint4(qk_pack(ol[0], ol[1]), qk_pack(ol[2], ol[3]), qk_pack(ol[4], ol[5]), qk_pack(ol[6], ol[7]));
-        wh = make_uint4(qk_pack(oh[0], oh[1]), qk_pack(oh[2], oh[3]), qk_pack(oh[4], oh[5]), qk_pack(oh[6], oh[7]));
+        wl = make_uint4(qk_pack(lo[0], lo[1]), qk_pack(lo[2], lo[3]), qk_pack(lo[4], lo[5]), qk_pack(lo[6], lo[7]));
+        wh = make_uint4(qk_pack(hi[0], hi[1]), qk_pack(hi[2], hi[3]), qk_pack(hi[4], hi[5]), qk_pack(hi[6], hi[7]));
       }
-      bf16* dst;
-      if (is_q) {
-        dst = a.q_out + r * a.q_stride + h * D + piece;
-      } else {
-        if (!cached) continue;
-        const int kvh = is_v ? h - a.heads - a.kv_heads : h - a.heads;
-        dst = (is_v ? a.values : a.keys) + at + kvh * a.head_stride + piece;
-      }
-      *reinterpret_cast<uint4*>(dst) = wl;
-      *reinterpret_cast<uint4*>(dst + HALF) = wh;
+      if (!live || (!is_q && !cached)) return;
+      bf16* dst = is_q ? a.q_out + r * a.q_stride + h * D
+                       : (is_v ? a.values + (h - a.heads - a.kv_heads) * a.head_stride
+                               : a.keys + (h - a.heads) * a.head_stride) + at;
+      *reinterpret_cast<uint4*>(dst + piece) = wl;
+      *reinterpret_cast<uint4*>(dst + piece + HALF) = wh;
+    };
+#pragma unroll
+    for (int k = 0; k < kQkAhead; ++k) {
+      if (k * kQkThreads < items) work(tid + k * kQkThreads, now[k]);
+    }
+    for (int first = kQkAhead * kQkThreads; first < items; first += kQkThreads) {  // wider rows
+      uint4 v[2];
+      fetch(r, first + tid, v);
+      work(first + tid, v);
     }
   }
 }

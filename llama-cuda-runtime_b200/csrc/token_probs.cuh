@@ -46,7 +46,7 @@ __device__ __forceinline__ unsigned long long probs_key(float x, int i) {
 // A slice beyond kProbsSlice ids (vocabularies beyond 8 x 16384) is gone over
 // again in memory.
 template <bool VEC>
-__global__ void __launch_bounds__(kProbsThreads) token_probs_kernel(const TokenProbsArgs a) {
+__global__ void __launch_bounds__(kProbsThreads, 2) token_probs_kernel(const TokenProbsArgs a) {
   const auto cluster = cooperative_groups::this_cluster();
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   __shared__ float red[2][kProbsThreads / 32];

@@ -27,15 +27,28 @@ struct VerifyArgs {
 };
 
 constexpr int kVerifyThreads = 512;
-constexpr int kVerifyCtas = 8;       // a cluster for each request
-constexpr int kVerifyChunks = 1024;  // of a CTA's slice, at most
+constexpr int kVerifyMaxCtas = 8;    // of a request's cluster
+constexpr int kVerifyChunks = 512;   // of a CTA's slice, at most
 constexpr int kVerifyElsewhere = -2; // verify_write: another CTA writes the drawn token
 constexpr long long kVerifyOne = 1ll << 38;
 
-// p in units of 2^-38. The scaling by a power of two is exact, so this is one
-// rounding (to nearest even), the same wherever it is done.
+// p in units of 2^-38, as h 2^22 + l: h = p 2^16 and l = the exact rest, both
+// rounded to whole numbers by adding 1.5 2^23, whose bits then carry them (less
+// kVerifyBias). h 2^22 is even, so ties fall as in one rounding to nearest even.
+// (A conversion to 64 bits has a fraction of the rate of these.)
+constexpr int kVerifyBias = 0x4B400000;
+struct VerifyFixed {
+  int h, l;  // biased
+};
+__device__ __forceinline__ VerifyFixed verify_split(float p) {
+  p = __saturatef(p);  // NaN becomes 0
+  const float t = __fmaf_rn(p, 65536.0f, 12582912.0f), h = __fsub_rn(t, 12582912.0f);
+  const float u = __fmaf_rn(__fmaf_rn(p, 65536.0f, -h), 4194304.0f, 12582912.0f);
+  return {__float_as_int(t), __float_as_int(u)};
+}
 __device__ __forceinline__ long long verify_fixed(float p) {
-  return __float2ll_rn(fminf(fmaxf(p, 0.f), 1.f) * 274877906944.0f);  // fmaxf drops a NaN
+  const VerifyFixed f = verify_split(p);
+  return static_cast<long long>(f.h - kVerifyBias) * 4194304ll + (f.l - kVerifyBias);
 }
 
 __device__ __forceinline__ unsigned long long verify_uniform(float u) {
@@ -73,6 +86,24 @@ __device__ __forceinline__ void verify_load(const VerifyRow& r, bool vec, int i,
     for (int e = 0; e < 4; ++e) {
       p[e] = i + e < end ? r.p[i + e] : 0.f;
       q[e] = i + e < end && r.q != nullptr ? r.q[i + e] : 0.f;
+    }
+  }
+}
+
+// Adds R of id i to (h, l). |l| of a difference is at most 2^22, so its sign
+// is h's, or l's where h is 0.
+__device__ __forceinline__ void verify_add(const VerifyRow& r, int i, float p, float q, int& h, int& l) {
+  const VerifyFixed x = verify_split(p);
+  if (r.q == nullptr) {
+    if (i == r.drafted) return;  // P - 1 is not above 0
+    h += x.h - kVerifyBias;
+    l += x.l - kVerifyBias;
+  } else {
+    const VerifyFixed y = verify_split(q);
+    const int dh = x.h - y.h, dl = x.l - y.l;
+    if (dh > 0 || (dh == 0 && dl > 0)) {
+      h += dh;
+      l += dl;
     }
   }
 }
@@ -118,21 +149,21 @@ __device__ __forceinline__ void verify_write(const VerifyArgs& a, int b, int kep
 }
 
 // Where the drawn token is in the row, by chunks of the vocabulary in order:
-// one cluster of eight CTAs takes a request, each CTA a contiguous slice in up
+// one cluster of up to eight CTAs takes a request, each a contiguous slice in up
 // to kVerifyChunks chunks, a warp a chunk at a time, so that the row (two rows
 // after a refusal) is read once. The CTAs exchange their slices' sums through
 // distributed shared memory; the one whose slice holds the target finds the
 // chunk and reads only that again. HBM bound for many requests; for one, a
 // chain of latencies (the draft, its two probabilities, the row, the exchange).
-__global__ void __cluster_dims__(kVerifyCtas, 1, 1) __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kVerifyThreads, 2) verify_drafts_kernel(const VerifyArgs a) {
   __shared__ int kept_s;
   __shared__ long long sums[kVerifyChunks];
-  __shared__ long long slice_s[2][kVerifyCtas];  // by pass
+  __shared__ long long slice_s[2][kVerifyMaxCtas];  // by pass
   __shared__ long long part[kVerifyThreads / 32];
   const auto cluster = cooperative_groups::this_cluster();
   cluster.barrier_arrive();  // this CTA runs: the others may write to its shared memory
-  const int rank = static_cast<int>(cluster.block_rank());
-  const int b = blockIdx.x / kVerifyCtas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int b = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r0 = a.target_starts[b], r1 = a.target_starts[b + 1];
   if (r1 <= r0) {  // the same for the whole cluster
     if (rank == 0) verify_write(a, b, -1, -1);
@@ -152,10 +183,11 @@ __global__ void __cluster_dims__(kVerifyCtas, 1, 1) __launch_bounds__(kVerifyThr
     else row.drafted = a.drafts[at];
   }
   const unsigned long long u = verify_uniform(a.uniforms[static_cast<size_t>(b) * (a.max_drafts + 1) + a.max_drafts]);
-  const int slice = (a.vocab + kVerifyCtas * 128 - 1) / (kVerifyCtas * 128) * 128;
+  const int slice = (a.vocab + ctas * 128 - 1) / (ctas * 128) * 128;
   const int i0 = min(a.vocab, rank * slice), i1 = min(a.vocab, i0 + slice);
-  // Chunks of a multiple of 128 ids: lane l has ids 4 l .. 4 l + 3 of each 128.
-  const int chunk = (slice + kVerifyChunks * 128 - 1) / (kVerifyChunks * 128) * 128;
+  // Chunks of 512 ids (a 64-bit sum over the lanes costs ten shuffles) or more:
+  // lane l has ids 4 l .. 4 l + 3 of each 128.
+  const int chunk = max(512, (slice + kVerifyChunks * 128 - 1) / (kVerifyChunks * 128) * 128);
   const int chunks = (i1 - i0 + chunk - 1) / chunk;
   int token = -1;
   cluster.barrier_wait();
@@ -163,38 +195,36 @@ __global__ void __cluster_dims__(kVerifyCtas, 1, 1) __launch_bounds__(kVerifyThr
     const bool vec = ((reinterpret_cast<uintptr_t>(row.p) | reinterpret_cast<uintptr_t>(row.q)) & 15u) == 0;
     long long mine = 0;
     constexpr int WARPS = kVerifyThreads / 32;
-    for (int c0 = warp; c0 < chunks; c0 += 4 * WARPS) {  // four chunks at a time, for their loads' sake
-      long long v[4] = {0, 0, 0, 0};
-      for (int o = 4 * lane; o < chunk; o += 128) {
+    for (int c = warp; c < chunks; c += WARPS) {
+      long long v = 0;
+      for (int o = 0; o < chunk; o += 512) {
+        const int i = i0 + c * chunk + o + 4 * lane;
         float p[4][4], q[4][4];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) verify_load(row, vec, i0 + (c0 + s * WARPS) * chunk + o, i1, p[s], q[s]);
+        for (int s = 0; s < 4; ++s) verify_load(row, vec, i + 128 * s, o + 128 * s < chunk ? i1 : 0, p[s], q[s]);
+        int h = 0, l = 0;  // of 16 ids: far from 2^31
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[s] += verify_residual(row, i0 + (c0 + s * WARPS) * chunk + o + e, p[s][e], q[s][e]);
+          for (int e = 0; e < 4; ++e) verify_add(row, i + 128 * s + e, p[s][e], q[s][e], h, l);
         }
+        v += static_cast<long long>(h) * 4194304ll + l;
       }
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-#pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) v[s] += __shfl_xor_sync(0xffffffffu, v[s], off);
-        if (c0 + s * WARPS < chunks) {
-          if (lane == 0) sums[c0 + s * WARPS] = v[s];
-          mine += v[s];
-        }
-      }
+      for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+      if (lane == 0) sums[c] = v;
+      mine += v;
     }
     if (lane == 0) part[warp] = mine;
     __syncthreads();
-    if (tid < kVerifyCtas) {
+    if (tid < ctas) {
       long long all = 0;
       for (int w = 0; w < WARPS; ++w) all += part[w];
       cluster.map_shared_rank(slice_s[pass], tid)[rank] = all;
     }
     cluster.sync();
     long long before = 0, total = 0;
-    for (int c = 0; c < kVerifyCtas; ++c) {
+    for (int c = 0; c < ctas; ++c) {
       if (c < rank) before += slice_s[pass][c];
       total += slice_s[pass][c];
     }
