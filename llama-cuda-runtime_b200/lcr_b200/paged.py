@@ -12,8 +12,9 @@ them together.
 
 Every function writes into tensors of the caller, on torch's current stream,
 and allocates nothing (``chunk_attention`` keeps one workspace for each device
-and stream unless it is given one). Tensors must be on torch's current
-device; int32 ones contiguous.
+and stream unless it is given one). Tensors must be on torch's current device;
+what does not fit raises ``ValueError`` (``csrc/tensors.cpp`` checks them), what
+the library refuses ``runtime.LcrError``.
 """
 from __future__ import annotations
 
@@ -24,9 +25,10 @@ import torch
 
 from . import runtime as rt
 
-_I32 = torch.int32
-_BF16 = torch.bfloat16
-_F32 = torch.float32
+try:
+    from ._tensors import pointers as _pointers
+except ImportError as e:  # like the library itself: no other path
+    raise RuntimeError(f"lcr_b200/_tensors.so is not built; run `make -C {rt.PKG_DIR}`") from e
 
 
 def _need(ok: bool, text: str) -> None:
@@ -34,41 +36,24 @@ def _need(ok: bool, text: str) -> None:
         raise ValueError(text)
 
 
-def _vector(t, n: int, name: str) -> int:
-    """Pointer of a contiguous int32 tensor of at least n elements."""
-    if t.dtype is not _I32 or not t.is_cuda or not t.is_contiguous() or t.numel() < n:
-        raise ValueError(f"{name}: a contiguous int32 CUDA tensor of {n} elements, got {t.dtype} {tuple(t.shape)} "
-                         f"on {t.device}")
-    return t.data_ptr()
-
-
-def _rows(t, dtype, name: str) -> int:
-    """Pointer of a 2-D tensor whose rows are dense."""
-    if t.dtype is not dtype or not t.is_cuda or t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
-        raise ValueError(f"{name}: a CUDA tensor of dense {dtype} rows, got {t.dtype} {tuple(t.shape)} with strides "
-                         f"{t.stride()} on {t.device}")
-    return t.data_ptr()
-
-
-def _stream(t) -> int:
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-    return torch.cuda.current_stream().cuda_stream
-
-
 def kv_view(keys, values, block_tables=None) -> rt.KvView:
     """The ``lcr_kv_view`` of a pair of pools [pages, kv_heads, page_size,
     head_dim] (any page and head strides, dense slots) and, for attention, the
     block tables."""
-    s = keys.stride()
-    if (keys.dtype is not _BF16 or values.dtype is not _BF16 or not keys.is_cuda or keys.dim() != 4
-            or keys.shape != values.shape or s != values.stride() or s[3] != 1 or s[2] != keys.shape[3]):
-        raise ValueError(f"keys and values: bf16 CUDA pools [pages, kv_heads, page_size, head_dim] with dense slots and "
-                         f"equal strides, got {keys.dtype} {tuple(keys.shape)} {s} and {values.dtype} "
-                         f"{tuple(values.shape)} {values.stride()}")
-    _need(s[0] < 2 ** 31 and s[1] < 2 ** 31, "page and head strides must fit in 31 bits")
-    return rt.KvView(keys.data_ptr(), values.data_ptr(), None if block_tables is None else block_tables.data_ptr(),
-                     keys.shape[2], s[0], s[1], keys.shape[1], keys.shape[3])
+    k, ps, hs, v, ps2, hs2, _ = _pointers(("keys", "values"), "KK", keys, 0, values, 0)
+    return _view(keys, values, k, ps, hs, v, ps2, hs2, None if block_tables is None else block_tables.data_ptr())
+
+
+def _view(keys, values, k, page_stride, head_stride, v, page_stride_v, head_stride_v, table) -> rt.KvView:
+    shape = keys.shape
+    _need(shape == values.shape and page_stride == page_stride_v and head_stride == head_stride_v,
+          "keys and values differ in shape or strides")
+    _need(page_stride < 2 ** 31 and head_stride < 2 ** 31, "page and head strides must fit in 31 bits")
+    return rt.KvView(k, v, table, shape[2], page_stride, head_stride, shape[1], shape[3])
+
+
+_PLAN = ("block_tables", "held", "held_out", "free_pages", "free_count", "free_count_out", "cached", "new_tokens",
+         "finished", "row_starts", "kv_lengths", "positions", "slots", "row_sequence")
 
 
 def plan_step(block_tables, held, free_pages, free_count, cached, new_tokens, finished=None, *, page_size: int,
@@ -77,17 +62,19 @@ def plan_step(block_tables, held, free_pages, free_count, cached, new_tokens, fi
     (``lcr_plan_step``). ``block_tables`` [requests, max_pages] and
     ``free_pages`` [pool pages] are updated in place; ``held_out`` may be
     ``held`` and ``free_count_out`` ``free_count``."""
-    _need(block_tables.dim() == 2, "block_tables: [requests, max_pages]")
     n, width = block_tables.shape
     rows = positions.numel()
-    rt.check(rt.lib().lcr_plan_step(
-        _vector(block_tables, n * width, "block_tables"), width, _vector(held, n, "held"),
-        _vector(held_out, n, "held_out"), _vector(free_pages, 1, "free_pages"), _vector(free_count, 1, "free_count"),
-        _vector(free_count_out, 1, "free_count_out"), free_pages.numel(), _vector(cached, n, "cached"),
-        _vector(new_tokens, n, "new_tokens"), None if finished is None else _vector(finished, n, "finished"), n,
-        page_size, rows, _vector(row_starts, n + 1, "row_starts"), _vector(kv_lengths, n, "kv_lengths"),
-        _vector(positions, rows, "positions"), _vector(slots, rows, "slots"),
-        _vector(row_sequence, rows, "row_sequence"), _stream(block_tables)))
+    (table, h, ho, stack, count, count_out, c, new, done, starts, kv, pos, slot, seq, stream) = _pointers(
+        _PLAN, "iiiiiiiiiiiiii", block_tables, n * width, held, n, held_out, n, free_pages, 1, free_count, 1,
+        free_count_out, 1, cached, n, new_tokens, n, finished, n, row_starts, n + 1, kv_lengths, n, positions, rows,
+        slots, rows, row_sequence, rows)
+    status = rt.lib().lcr_plan_step(table, width, h, ho, stack, count, count_out, free_pages.numel(), c, new, done, n,
+                                    page_size, rows, starts, kv, pos, slot, seq, stream)
+    if status:
+        rt.check(status)
+
+
+_ROPE = ("q_out", "keys", "values", "qkv", "positions", "slots", "inv_freq", "q_gain", "k_gain")
 
 
 def qk_norm_rope_kv(q_out, keys, values, qkv, positions, slots, inv_freq, q_gain=None, k_gain=None, *,
@@ -95,23 +82,20 @@ def qk_norm_rope_kv(q_out, keys, values, qkv, positions, slots, inv_freq, q_gain
     """Per-head norms of q and k (where a gain is given), rotary positions and
     the cache write of the rows of ``qkv`` [rows, (heads + 2 kv_heads) *
     head_dim] (``lcr_qk_norm_rope_kv``)."""
-    view = kv_view(keys, values)
-    d = view.head_dim
     rows, width = qkv.shape
-    heads = width // d - 2 * view.num_kv_heads
-    _need(heads > 0 and width % d == 0 and q_out.shape[0] == rows and q_out.shape[1] == heads * d,
-          f"qkv {tuple(qkv.shape)} and q_out {tuple(q_out.shape)} do not fit heads of {d} on {view.num_kv_heads} "
-          "KV heads")
-    _need(inv_freq.dtype is _F32 and inv_freq.is_cuda and inv_freq.is_contiguous() and inv_freq.numel() == d // 2,
-          "inv_freq: head_dim / 2 fp32 values")
-    for g in (q_gain, k_gain):
-        _need(g is None or (g.dtype is _BF16 and g.is_cuda and g.is_contiguous() and g.numel() == d),
-              "gains: head_dim bf16 values")
-    rt.check(rt.lib().lcr_qk_norm_rope_kv(
-        _rows(q_out, _BF16, "q_out"), q_out.stride(0), ctypes.byref(view), keys.shape[0], _rows(qkv, _BF16, "qkv"),
-        qkv.stride(0), rows, heads, None if q_gain is None else q_gain.data_ptr(),
-        None if k_gain is None else k_gain.data_ptr(), eps, inv_freq.data_ptr(), _vector(positions, rows, "positions"),
-        _vector(slots, rows, "slots"), _stream(qkv)))
+    pages, kv_heads, _, d = keys.shape
+    heads = width // d - 2 * kv_heads
+    _need(heads > 0 and width % d == 0 and q_out.shape[0] == rows and inv_freq.numel() == d // 2,
+          f"qkv {tuple(qkv.shape)}, q_out {tuple(q_out.shape)} and inv_freq {tuple(inv_freq.shape)} do not fit heads "
+          f"of {d} on {kv_heads} KV heads")
+    (q, q_stride, k, ps, hs, v, ps2, hs2, x, x_stride, pos, slot, freq, gq, gk, stream) = _pointers(
+        _ROPE, "HKKHiifhh", q_out, heads * d, keys, 0, values, 0, qkv, width, positions, rows, slots, rows, inv_freq,
+        d // 2, q_gain, d, k_gain, d)
+    view = _view(keys, values, k, ps, hs, v, ps2, hs2, None)
+    status = rt.lib().lcr_qk_norm_rope_kv(q, q_stride, ctypes.byref(view), pages, x, x_stride, rows, heads, gq or None,
+                                          gk or None, eps, freq, pos, slot, stream)
+    if status:
+        rt.check(status)
 
 
 _workspaces: dict = {}
@@ -123,28 +107,34 @@ def attention_workspace(heads: int, head_dim: int, device=None) -> torch.Tensor:
                        device=device if device is not None else torch.cuda.current_device())
 
 
+_ATTENTION = ("out", "q", "keys", "values", "block_tables", "row_starts", "kv_lengths")
+
+
 def chunk_attention(out, q, keys, values, block_tables, row_starts, kv_lengths, *, scale: float,
                     workspace: Optional[torch.Tensor] = None) -> None:
     """Attention of each request's new rows (``q`` [rows, heads * head_dim],
     packed) over its pages (``lcr_chunk_attention``)."""
-    view = kv_view(keys, values, block_tables)
     rows, width = q.shape
     n = kv_lengths.numel()
-    heads = width // view.head_dim
-    _need(width == heads * view.head_dim and out.shape == q.shape, f"q {tuple(q.shape)} and out {tuple(out.shape)} do "
-          f"not fit heads of {view.head_dim}")
-    _need(block_tables.dim() == 2 and block_tables.shape[0] >= n, "block_tables: [requests, max_pages]")
-    stream = _stream(q)
+    requests, max_pages = block_tables.shape
+    d = keys.shape[3]
+    heads = width // d
+    _need(width == heads * d and out.shape[0] == rows and requests >= n,
+          f"q {tuple(q.shape)}, out {tuple(out.shape)} and block_tables {tuple(block_tables.shape)} do not fit {n} "
+          f"requests and heads of {d}")
+    (o, o_stride, x, x_stride, k, ps, hs, v, ps2, hs2, table, starts, kv, stream) = _pointers(
+        _ATTENTION, "HHKKiii", out, width, q, width, keys, 0, values, 0, block_tables, requests * max_pages, row_starts,
+        n + 1, kv_lengths, n)
     if workspace is None:
-        key = (q.device.index, stream, heads, view.head_dim)
+        key = (q.get_device(), stream, d)
         workspace = _workspaces.get(key)
         if workspace is None:
-            workspace = _workspaces[key] = attention_workspace(heads, view.head_dim)
-    _vector(block_tables, 1, "block_tables")
-    rt.check(rt.lib().lcr_chunk_attention(
-        _rows(out, _BF16, "out"), out.stride(0), _rows(q, _BF16, "q"), q.stride(0), ctypes.byref(view),
-        block_tables.shape[1], keys.shape[0], _vector(row_starts, n + 1, "row_starts"),
-        _vector(kv_lengths, n, "kv_lengths"), n, rows, heads, scale, workspace.data_ptr(), workspace.numel(), stream))
+            workspace = _workspaces[key] = attention_workspace(heads, d)
+    view = _view(keys, values, k, ps, hs, v, ps2, hs2, table)
+    status = rt.lib().lcr_chunk_attention(o, o_stride, x, x_stride, ctypes.byref(view), max_pages, keys.shape[0], starts,
+                                          kv, n, rows, heads, scale, workspace.data_ptr(), workspace.numel(), stream)
+    if status:
+        rt.check(status)
 
 
 def attention_status(workspace: Optional[torch.Tensor] = None) -> None:
@@ -157,34 +147,38 @@ def attention_status(workspace: Optional[torch.Tensor] = None) -> None:
         rt.check(rt.lib().lcr_chunk_attention_status(w.data_ptr(), stream))
 
 
+_PROBS = ("probs", "logits", "temperature", "row_sequence")
+
+
 def token_probs(probs, logits, temperature=None, row_sequence=None) -> None:
     """Rows of fp32 logits to rows of probabilities (``lcr_token_probs``), by
-    the temperature of each row, or of each row's request."""
-    _need(probs.shape == logits.shape, "probs and logits have the same shape")
+    the temperature of each row, or of each row's request (an entry of
+    ``row_sequence`` past ``temperature`` is not checked)."""
     rows, vocab = logits.shape
-    _need(temperature is None or (temperature.dtype is _F32 and temperature.is_cuda and temperature.is_contiguous()
-                                  and (row_sequence is not None or temperature.numel() >= rows)),
-          "temperature: one fp32 value for each row (or request, with row_sequence)")
-    rt.check(rt.lib().lcr_token_probs(
-        _rows(probs, _F32, "probs"), probs.stride(0), _rows(logits, _F32, "logits"), logits.stride(0), rows, vocab,
-        None if temperature is None else temperature.data_ptr(),
-        None if row_sequence is None else _vector(row_sequence, rows, "row_sequence"), _stream(logits)))
+    _need(probs.shape[0] == rows, "probs and logits have the same shape")
+    p, p_stride, x, x_stride, t, seq, stream = _pointers(
+        _PROBS, "FFfi", probs, vocab, logits, vocab, temperature, 1 if row_sequence is not None else rows, row_sequence,
+        rows)
+    status = rt.lib().lcr_token_probs(p, p_stride, x, x_stride, rows, vocab, t or None, seq or None, stream)
+    if status:
+        rt.check(status)
+
+
+_VERIFY = ("tokens", "accepted", "target_probs", "target_starts", "drafts", "draft_counts", "draft_probs", "uniforms")
 
 
 def verify_drafts(tokens, accepted, target_probs, target_starts, drafts, draft_counts, draft_probs, uniforms) -> None:
     """Keeps each request's drafts as far as the given uniforms allow and draws
     its next token (``lcr_verify_drafts``). ``draft_probs`` [requests,
     max_drafts, vocab], or None for drafts that were certain."""
-    _need(drafts.dim() == 2 and tokens.dim() == 2, "drafts: [requests, max_drafts], tokens: [requests, max_drafts + 1]")
     n, k = drafts.shape
-    _need(tokens.shape[0] == n and tokens.shape[1] == k + 1, "tokens: [requests, max_drafts + 1]")
-    _need(uniforms.dtype is _F32 and uniforms.is_cuda and uniforms.is_contiguous() and uniforms.shape == tokens.shape,
-          "uniforms: fp32 [requests, max_drafts + 1]")
     vocab = target_probs.shape[1]
-    _need(draft_probs is None or (draft_probs.dtype is _F32 and draft_probs.is_cuda and draft_probs.is_contiguous()
-                                  and draft_probs.shape == (n, k, vocab)), "draft_probs: fp32 [requests, max_drafts, vocab]")
-    rt.check(rt.lib().lcr_verify_drafts(
-        _vector(tokens, n * (k + 1), "tokens"), _vector(accepted, n, "accepted"),
-        _rows(target_probs, _F32, "target_probs"), target_probs.stride(0), _vector(target_starts, n + 1, "target_starts"),
-        _vector(drafts, n * k, "drafts"), _vector(draft_counts, n, "draft_counts"),
-        None if draft_probs is None else draft_probs.data_ptr(), uniforms.data_ptr(), n, k, vocab, _stream(tokens)))
+    _need(tokens.shape == (n, k + 1) and uniforms.shape == tokens.shape,
+          "tokens and uniforms: [requests, max_drafts + 1]")
+    _need(draft_probs is None or draft_probs.shape == (n, k, vocab), "draft_probs: [requests, max_drafts, vocab]")
+    t, got, p, p_stride, starts, d, counts, q, u, stream = _pointers(
+        _VERIFY, "iiFiiiff", tokens, n * (k + 1), accepted, n, target_probs, vocab, target_starts, n + 1, drafts, n * k,
+        draft_counts, n, draft_probs, n * k * vocab, uniforms, n * (k + 1))
+    status = rt.lib().lcr_verify_drafts(t, got, p, p_stride, starts, d, counts, q or None, u, n, k, vocab, stream)
+    if status:
+        rt.check(status)

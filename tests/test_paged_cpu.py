@@ -74,5 +74,5 @@ def test_probs_and_verify_refuse(L):
 
 
 def test_scratch_size(L):
-    assert L.lcr_chunk_attention_scratch_bytes(32, 64) > 0
-    assert L.lcr_chunk_attention_scratch_bytes(32, 128) >= L.lcr_chunk_attention_scratch_bytes(32, 64)
+    assert 0 < L.lcr_chunk_attention_scratch_bytes(32, 64) < 1 << 28
+    assert 0 < L.lcr_chunk_attention_scratch_bytes(32, 128) < 1 << 28

@@ -419,6 +419,32 @@ def test_chunk_attention_lengths_past_the_tables():
     assert bool(((got.double() - want).abs() <= bound).all())
 
 
+@pytest.mark.parametrize("ps", [16, 5])
+def test_offsets_past_32_bits(ps):
+    """Pools of more than 2^31 elements: rows are written to and read from
+    their last pages (page sizes with and without tensor copies)."""
+    kv_heads, d, heads = 8, 64, 16
+    pages = (2 ** 31 + 2 ** 28) // (kv_heads * ps * d)
+    keys = torch.empty(pages, kv_heads, ps, d, dtype=torch.bfloat16, device=DEV)
+    values = torch.empty_like(keys)
+    n, g = 37, torch.Generator(device=DEV).manual_seed(21)
+    used = -(-n // ps)
+    table = torch.arange(pages - used, pages, dtype=torch.int32, device=DEV).flip(0)[None].contiguous()
+    assert (pages - used) * kv_heads * ps * d > 2 ** 31
+    pos = torch.arange(n, dtype=torch.int32, device=DEV)
+    slots = table[0, (pos // ps).long()] * ps + pos % ps
+    qkv = torch.randn(n, (heads + 2 * kv_heads) * d, generator=g, device=DEV).bfloat16()
+    q = torch.empty(n, heads * d, dtype=torch.bfloat16, device=DEV)
+    paged.qk_norm_rope_kv(q, keys, values, qkv, torch.zeros_like(pos), slots, torch.ones(d // 2, device=DEV))
+    assert torch.equal(q, qkv[:, :heads * d])  # position 0: no turn
+    c = dict(q=q, keys=keys, values=values, tables=table, starts=i32([0, n]), kv=i32([n]), lens=[(n, n)], heads=heads,
+             kv_heads=kv_heads, d=d, ps=ps, host_tables=table.cpu().numpy(), host_starts=np.array([0, n]))
+    flat = qkv.view(n, -1, d)
+    assert torch.equal(keys[table[0].long()].permute(0, 2, 1, 3).reshape(-1, kv_heads, d)[:n], flat[:, heads:heads + kv_heads])
+    assert torch.equal(values[table[0].long()].permute(0, 2, 1, 3).reshape(-1, kv_heads, d)[:n], flat[:, heads + kv_heads:])
+    check_attention(c)
+
+
 # ---------------------------------------------------------------------------
 # token_probs
 # ---------------------------------------------------------------------------
