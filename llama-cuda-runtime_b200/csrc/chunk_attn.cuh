@@ -56,9 +56,21 @@ namespace lcrb {
 
 constexpr int kCaThreads = 192;
 constexpr int kCaRows = 128;      // (row, head) pairs per tile
-constexpr int kCaTileCost = 3;    // units a tile's start and end count for, beside one for each block
-constexpr int kCaSnap = 4;        // units from a tile's end within which a range's end moves there
-constexpr int kCaMinRange = 4;    // units of a range at least (where there are as many); at least kCaSnap
+// In units of a block of BLK keys (64 or 128); chosen by timing 64 requests of 1
+// - 5 rows on 128 - 4096 keys (BLK 64: 77, 71, 71 us at a cost of 2, 3, 4) and a
+// chunk of 509 rows beside 15 such requests (BLK 128: 49, 45 us at a reach of 2, 3).
+template <int BLK>
+constexpr int ca_tile_cost() {  // what a tile's start and end count for
+  return BLK == 64 ? 3 : 2;
+}
+template <int BLK>
+constexpr int ca_reach() {  // a range's end moves to a tile's end this near
+  return BLK == 64 ? 4 : 3;
+}
+template <int BLK>
+constexpr int ca_min_range() {  // units of a range at least (where there are as many); at least ca_reach
+  return ca_reach<BLK>();
+}
 constexpr int kCaFmaGroups = 1;   // of 8 pairs of exponentials, on the FMA pipe
 
 struct ChunkAttnArgs {
@@ -120,13 +132,13 @@ __device__ __forceinline__ int ca_blocks_before(int s, int t, int log2_qb) {
   return static_cast<int>(below(a1 + n + 1) - below(a1 + 1));
 }
 
-// Ranges are cut in units of blocks with kCaTileCost units added in front of
+// Ranges are cut in units of blocks with ca_tile_cost units added in front of
 // every tile, about what a change of tiles costs (Q, the first S, the
 // epilogue): a range with many short tiles gets fewer blocks.
 
 template <int BLK>
 __device__ __forceinline__ int ca_units_before(int s, int t, int log2_qb) {
-  return ca_blocks_before<BLK>(s, t, log2_qb) + t * kCaTileCost;
+  return ca_blocks_before<BLK>(s, t, log2_qb) + t * ca_tile_cost<BLK>();
 }
 
 // One request as the kernel sees it: malformed lengths are cut to what the
@@ -148,7 +160,7 @@ __device__ __forceinline__ CaSeq ca_seq(const ChunkAttnArgs& a, int b) {
   q.s = max(0, q.kv - q.n);
   q.tiles = (q.n + (1 << a.log2_qb) - 1) >> a.log2_qb;
   q.units = q.tiles == 0 ? 0
-                         : ca_units_before<BLK>(q.s, q.tiles - 1, a.log2_qb) + (q.s + q.n + BLK - 1) / BLK + kCaTileCost;
+                         : ca_units_before<BLK>(q.s, q.tiles - 1, a.log2_qb) + (q.s + q.n + BLK - 1) / BLK + ca_tile_cost<BLK>();
   return q;
 }
 
@@ -192,9 +204,9 @@ struct CaWalk {
     q = ca_seq<BLK>(a, b);
     len = ca_tile_len<BLK>(q, t, a.log2_qb);
   }
-  __device__ __forceinline__ int units() const { return min(len + kCaTileCost - at, left); }
-  __device__ __forceinline__ int off() const { return max(0, at - kCaTileCost); }  // first block of the segment
-  __device__ __forceinline__ int count() const { return max(0, at + units() - kCaTileCost) - off(); }  // its blocks
+  __device__ __forceinline__ int units() const { return min(len + ca_tile_cost<BLK>() - at, left); }
+  __device__ __forceinline__ int off() const { return max(0, at - ca_tile_cost<BLK>()); }  // first block of the segment
+  __device__ __forceinline__ int count() const { return max(0, at + units() - ca_tile_cost<BLK>()) - off(); }  // its blocks
   // Keys the tile's last row sees, of those cached.
   __device__ __forceinline__ int key_end(const ChunkAttnArgs& a) const {
     return max(0, q.kv - q.n + min(q.n, (t + 1) << a.log2_qb));
@@ -223,17 +235,17 @@ struct CaWalk {
 };
 
 // How far an end of a range that lies `at` units into a tile of `units` moves:
-// splitting a tile costs its CTAs about as much as kCaSnap units (a part stored,
-// counted and joined). Ends are at least kCaSnap apart, so that only one of a
+// splitting a tile costs its CTAs about as much as `reach` units (a part stored,
+// counted and joined). Ends are at least `reach` apart, so that only one of a
 // tile's moves to each of its own ends.
-__device__ __forceinline__ int ca_snap(int at, int units) {
-  return at <= kCaSnap ? -at : units - at <= kCaSnap ? units - at : 0;
+__device__ __forceinline__ int ca_snap(int at, int units, int reach) {
+  return at <= reach ? -at : units - at <= reach ? units - at : 0;
 }
 // The range that unit `y` of the tile [begin, begin + units) falls to.
-__device__ __forceinline__ int ca_owner(int y, int begin, int units, int per) {
+__device__ __forceinline__ int ca_owner(int y, int begin, int units, int per, int reach) {
   const int c = y / per, from = c * per - begin, to = from + per;
-  if (from > 0 && ca_snap(from, units) > 0) return c - 1;
-  if (to < units && ca_snap(to, units) < 0) return c + 1;
+  if (from > 0 && ca_snap(from, units, reach) > 0) return c - 1;
+  if (to < units && ca_snap(to, units, reach) < 0) return c + 1;
   return c;
 }
 
@@ -457,7 +469,7 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
                                                                                 const __grid_constant__ CUtensorMap kmap,
                                                                                 const __grid_constant__ CUtensorMap vmap) {
   using G = CaGeom<D>;
-  constexpr int SLOTS = G::SLOTS, BLOCK = G::BLOCK;
+  constexpr int SLOTS = G::SLOTS, BLOCK = G::BLOCK, COST = ca_tile_cost<BLOCK>();
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* qs = smem;
   uint8_t* ring = smem + G::Q_BYTES;
@@ -528,7 +540,7 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
     total += p;
   }
   // As many ranges as CTAs, fewer where each would be short.
-  const int ranges = min(static_cast<int>(gridDim.x), max(1, total / kCaMinRange));
+  const int ranges = min(static_cast<int>(gridDim.x), max(1, total / ca_min_range<BLOCK>()));
   const int per = (total + ranges - 1) / ranges;
   const int c = blockIdx.x;
   // Both ends, snapped; the thread whose requests hold an end finds it.
@@ -545,7 +557,7 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
       }
       CaWalk<BLOCK> e;
       e.find(a, b, at);
-      const int shift = ca_snap(e.at, e.len + kCaTileCost);
+      const int shift = ca_snap(e.at, e.len + COST, ca_reach<BLOCK>());
       const int edge = static_cast<int>(raw) + shift;
       st->edge[k] = edge;
       if (k == 0) {
@@ -945,8 +957,9 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
           }
         }
         // The ranges of the tile's first and last block.
-        const int tile0 = done - w.at, units = w.len + kCaTileCost;
-        const int c0 = ca_owner(tile0 + kCaTileCost, tile0, units, per), c1 = ca_owner(tile0 + units - 1, tile0, units, per);
+        const int tile0 = done - w.at, units = w.len + COST;
+        const int c0 = ca_owner(tile0 + COST, tile0, units, per, ca_reach<BLOCK>()),
+                  c1 = ca_owner(tile0 + units - 1, tile0, units, per, ca_reach<BLOCK>());
         __syncwarp();
         if (lane == 0) mbar_arrive(stored);
         ok = __all_sync(0xffffffffu, ca_wait(stored, parts & 1, a.status, kStatusTimeoutFull));

@@ -234,11 +234,11 @@ extern "C" int lcr_chunk_attention(void* out, int64_t out_stride, const void* q,
   a.partials = reinterpret_cast<float*>(work + attention_header(static_cast<size_t>(ctas)));
   // As many CTAs as the tables' capacity could give ranges.
   const double tiles = a.kv_heads * (std::ldexp(static_cast<double>(rows), -a.log2_qb) + sequences);
-  const double blocks = tiles * ((static_cast<double>(max_pages) * view->page_size + rows) / view->head_dim + 1 + kCaTileCost);
+  const double blocks = tiles * ((static_cast<double>(max_pages) * view->page_size + rows) / view->head_dim + 1 + ca_tile_cost<64>());
   LCRB_REQUIRE(blocks < 2147483647.0, LCR_ERR_SHAPE,
                "chunk_attention: %d rows of %d requests over tables of %d positions are too many blocks", rows, sequences,
                max_pages * view->page_size);
-  const int grid = static_cast<int>(std::min(static_cast<double>(ctas), std::max(1.0, blocks / kCaMinRange)));
+  const int grid = static_cast<int>(std::min(static_cast<double>(ctas), std::max(1.0, blocks / ca_min_range<128>())));
   return view->head_dim == 64 ? chunk_attention<64>(a, grid, cs(stream)) : chunk_attention<128>(a, grid, cs(stream));
 }
 
