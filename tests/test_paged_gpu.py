@@ -222,7 +222,7 @@ def test_qk_norm_rope_kv_in_place():
     paged.qk_norm_rope_kv(out, keys, values, qkv, *args)
     L = rt.lib()
     import ctypes
-    view = paged.kv_view(k2, v2)
+    view = rt.KvView(k2.data_ptr(), v2.data_ptr(), None, 16, 2 * 16 * 64, 16 * 64, 2, 64)
     rt.check(L.lcr_qk_norm_rope_kv(qkv.data_ptr(), 512, ctypes.byref(view), 4, qkv.data_ptr(), 512, 9, 4, None, None,
                                    1e-5, args[2].data_ptr(), args[0].data_ptr(), args[1].data_ptr(), rt.stream_ptr()))
     assert torch.equal(qkv[:, :256], out) and torch.equal(keys, k2) and torch.equal(values, v2)
