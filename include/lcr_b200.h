@@ -426,7 +426,8 @@ LCR_API int lcr_batch_time_steps(lcr_batch* batch, int steps, float* ms);
 /* packed: request b owns rows row_starts[b] .. row_starts[b + 1] - 1. The     */
 /* cache is an lcr_kv_view whose keys / values are pools of pool_pages pages:  */
 /* page p, KV head h, slot s at p * page_stride + h * head_stride + s *        */
-/* head_dim elements (64-bit offsets; the strides multiples of 8 elements);    */
+/* head_dim elements (the strides multiples of 8 elements; the pool, up to     */
+/* 2^35 elements, passes 32-bit offsets);                                      */
 /* view->page_table is the requests' tables, [sequences][max_pages] physical   */
 /* pages. Any page_size from 1 up.                                             */
 /* ------------------------------------------------------------------------- */
@@ -453,7 +454,9 @@ LCR_API int lcr_batch_time_steps(lcr_batch* batch, int steps, float* ms);
  * held and free_count themselves), row_starts [sequences + 1], kv_lengths
  * [sequences] (cached + new, 0 if refused), and for each row r < max_rows its
  * positions[r], slots[r] = page * page_size + position % page_size (-1 if
- * refused) and row_sequence[r] = b. Rows past max_rows are cut off.
+ * refused) and row_sequence[r] = b. Rows past max_rows are cut off; those
+ * left over below it get 0, -1 and -1, so that a step captured in a graph for
+ * max_rows rows runs with fewer.
  * pool_pages * page_size must fit in 31 bits. */
 LCR_API int lcr_plan_step(int32_t* block_tables, int max_pages, const int32_t* held, int32_t* held_out,
                           int32_t* free_pages, const int32_t* free_count, int32_t* free_count_out,
@@ -481,8 +484,8 @@ LCR_API int lcr_qk_norm_rope_kv(void* q_out, int64_t q_stride, const lcr_kv_view
 /* Attention of every request's new rows over its pages. Row i of the n rows
  * of request b sits at position p = kv_lengths[b] - n + i and attends to the
  * cached positions 0 .. p (its own and earlier new tokens' K / V are in the
- * cache already): out = softmax(scale * q k) v, query head h on KV head
- * h / (num_heads / num_kv_heads). A row with no position (p < 0, e.g. of a
+ * cache already): out = softmax(scale * q k) v with scale > 0, query head h on
+ * KV head h / (num_heads / num_kv_heads). A row with no position (p < 0, e.g. of a
  * refused request) gives zeros. head_dim 64 or 128, any number of query heads
  * per KV head up to 128. q and out: [rows][num_heads * head_dim] with row
  * strides in elements (multiples of 8), 16-byte aligned, not overlapping.
@@ -507,12 +510,13 @@ LCR_API int lcr_chunk_attention_status(void* scratch, lcr_stream_t stream);
 
 /* Rows of fp32 logits to probabilities: probs = softmax(logits / t) with t =
  * temperature[row_sequence[r]] (row_sequence NULL: temperature[r];
- * temperature NULL: 1); t <= 0 puts everything on the largest logit (lowest
- * id on ties). Logits of -inf get 0, and a row of nothing but -inf is all
- * zeros. probs may be logits itself. Row strides in elements. */
+ * temperature NULL: 1), of which there are temperatures; t <= 0 puts
+ * everything on the largest logit (lowest id on ties). Logits of -inf get 0;
+ * a row of nothing but -inf, or of a request outside the temperatures (-1), is
+ * all zeros. probs may be logits itself. Row strides in elements. */
 LCR_API int lcr_token_probs(float* probs, int64_t probs_stride, const float* logits, int64_t logits_stride,
-                            int rows, int vocab, const float* temperature, const int32_t* row_sequence,
-                            lcr_stream_t stream);
+                            int rows, int vocab, const float* temperature, int temperatures,
+                            const int32_t* row_sequence, lcr_stream_t stream);
 
 /* Verification of drafted tokens by given random numbers, so that the tokens
  * kept are distributed as the target's own samples.

@@ -50,10 +50,11 @@ int multiprocessors() {
 
 // A launch in clusters of `ctas` CTAs along x.
 template <class Args>
-int launch_cluster(void (*kernel)(Args), int grid, int ctas, int threads, cudaStream_t s, const Args& args) {
+int launch_cluster(void (*kernel)(Args), int grid, int ctas, int threads, size_t smem, cudaStream_t s, const Args& args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -256,22 +257,26 @@ extern "C" int lcr_chunk_attention_status(void* scratch, lcr_stream_t stream) {
 }
 
 extern "C" int lcr_token_probs(float* probs, int64_t probs_stride, const float* logits, int64_t logits_stride, int rows,
-                               int vocab, const float* temperature, const int32_t* row_sequence, lcr_stream_t stream) {
+                               int vocab, const float* temperature, int temperatures, const int32_t* row_sequence,
+                               lcr_stream_t stream) {
   if (rows == 0) return LCR_OK;
   LCRB_REQUIRE(probs && logits && rows > 0 && vocab > 0, LCR_ERR_INVALID, "token_probs: null pointer or bad size");
   LCRB_REQUIRE(probs_stride >= vocab && logits_stride >= vocab, LCR_ERR_INVALID,
                "token_probs: row strides %lld and %lld of %d ids", static_cast<long long>(probs_stride),
                static_cast<long long>(logits_stride), vocab);
-  TokenProbsArgs a = {probs, probs_stride, logits, logits_stride, rows, vocab, temperature, row_sequence, 0};
-  // CTAs for a row: enough to keep it in registers, and for few rows as many as
-  // fill the GPU (one row of 128256 ids: 8 CTAs).
+  LCRB_REQUIRE(temperature == nullptr || temperatures >= (row_sequence != nullptr ? 1 : rows), LCR_ERR_INVALID,
+               "token_probs: %d temperatures of %d rows", temperatures, rows);
+  TokenProbsArgs a = {probs, probs_stride, logits, logits_stride, rows, vocab, temperature, temperatures, row_sequence, 0};
+  // CTAs for a row: enough to keep it in shared memory, and for few rows as many
+  // as fill the GPU (one row of 128256 ids: 8 CTAs).
   int ctas = 1;
   while (ctas < kProbsMaxCtas && (vocab > ctas * kProbsSlice || (rows * ctas < 256 && vocab > ctas * 2048))) ctas *= 2;
   LCRB_REQUIRE(rows <= INT32_MAX / ctas, LCR_ERR_SHAPE, "token_probs: %d rows", rows);
   a.slice = ((vocab + ctas - 1) / ctas + 3) / 4 * 4;
   const bool vec = aligned16(probs) && aligned16(logits) && probs_stride % 4 == 0 && logits_stride % 4 == 0;
-  return launch_cluster(vec ? token_probs_kernel<true> : token_probs_kernel<false>, rows * ctas, ctas, kProbsThreads,
-                        cs(stream), a);
+  const auto kernel = vec ? token_probs_kernel<true> : token_probs_kernel<false>;
+  LCRB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kProbsSlice * 4));
+  return launch_cluster(kernel, rows * ctas, ctas, kProbsThreads, sizeof(float) * std::min(a.slice, kProbsSlice), cs(stream), a);
 }
 
 extern "C" int lcr_verify_drafts(int32_t* tokens, int32_t* accepted, const float* target_probs, int64_t target_stride,
@@ -289,5 +294,5 @@ extern "C" int lcr_verify_drafts(int32_t* tokens, int32_t* accepted, const float
   // CTAs for a request: as many as run at once (two on an SM) for all of them.
   int ctas = 1;
   while (ctas < kVerifyMaxCtas && static_cast<long long>(sequences) * ctas * 2 <= 296) ctas *= 2;
-  return launch_cluster(verify_drafts_kernel, sequences * ctas, ctas, kVerifyThreads, cs(stream), a);
+  return launch_cluster(verify_drafts_kernel, sequences * ctas, ctas, kVerifyThreads, 0, cs(stream), a);
 }

@@ -248,6 +248,12 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
       }
     }
   }
+  // The rows left over, for steps of a fixed number of rows: nobody's.
+  for (int r = total + me; r < a.max_rows; r += kAll) {
+    a.positions[r] = 0;
+    a.slots[r] = -1;
+    a.row_sequence[r] = -1;
+  }
 }
 
 }  // namespace lcrb

@@ -74,6 +74,7 @@ class Call {
   T* maybe(int i, const char* name, at::ScalarType type, int64_t n) {
     return args_[i] == Py_None ? nullptr : flat<T>(i, name, type, n);
   }
+  int64_t numel(int i) { return THPVariable_Unpack(args_[i]).numel(); }
   int32_t* ints(int i, const char* name, int64_t n) { return flat<int32_t>(i, name, at::kInt, n); }
   // Rows of dense elements.
   const at::Tensor& rows(int i, const char* name, at::ScalarType type) {
@@ -196,9 +197,10 @@ int token_probs(PyObject* const* args, Py_ssize_t nargs) {
   Call::fits(p.sizes() == x.sizes(), "probs and logits have the same shape");
   const int rows = c.small(x.size(0));
   const int32_t* seq = c.maybe<int32_t>(3, "row_sequence", at::kInt, rows);
+  const float* t = c.maybe<float>(2, "temperature", at::kFloat, seq != nullptr ? 1 : rows);
+  const int temperatures = t != nullptr ? c.small(c.numel(2)) : 0;
   return token_probs_c(static_cast<float*>(p.data_ptr()), p.stride(0), static_cast<const float*>(x.data_ptr()), x.stride(0),
-                       rows, c.small(x.size(1)), c.maybe<float>(2, "temperature", at::kFloat, seq != nullptr ? 1 : rows), seq,
-                       c.stream());
+                       rows, c.small(x.size(1)), t, temperatures, seq, c.stream());
 }
 
 // (tokens, accepted, target_probs, target_starts, drafts, draft_counts,

@@ -48,7 +48,7 @@ def plan_step(block_tables, held, free_pages, free_count, cached, new_tokens, fi
     (``lcr_plan_step``). ``block_tables`` [requests, max_pages] and
     ``free_pages`` [pool pages] are updated in place; ``held_out`` may be
     ``held`` and ``free_count_out`` ``free_count``. The step has
-    ``positions.numel()`` rows at most."""
+    ``positions.numel()`` rows at most; those left over belong to nobody."""
     status = (_lib or _operators()).plan_step(block_tables, held, free_pages, free_count, cached, new_tokens, finished,
                                               page_size, held_out, free_count_out, row_starts, kv_lengths, positions,
                                               slots, row_sequence)
@@ -103,8 +103,8 @@ def attention_status(workspace: Optional[torch.Tensor] = None) -> None:
 
 def token_probs(probs, logits, temperature=None, row_sequence=None) -> None:
     """Rows of fp32 logits to rows of probabilities (``lcr_token_probs``), by
-    the temperature of each row, or of each row's request (an entry of
-    ``row_sequence`` past ``temperature`` is not checked)."""
+    the temperature of each row, or of each row's request (zeros for a row of
+    no request: an entry of ``row_sequence`` outside ``temperature``)."""
     status = (_lib or _operators()).token_probs(probs, logits, temperature, row_sequence)
     if status:
         rt.check(status)

@@ -170,7 +170,7 @@ _SIGS = {
                                  ctypes.c_size_t, _V]),
     "lcr_chunk_attention_scratch_bytes": (ctypes.c_size_t, [_I, _I]),
     "lcr_chunk_attention_status": (_I, [_V, _V]),
-    "lcr_token_probs": (_I, [_V, _L, _V, _L, _I, _I, _V, _V, _V]),
+    "lcr_token_probs": (_I, [_V, _L, _V, _L, _I, _I, _V, _I, _V, _V]),
     "lcr_verify_drafts": (_I, [_V, _V, _V, _L, _V, _V, _V, _V, _V, _I, _I, _I, _V]),
 }
 

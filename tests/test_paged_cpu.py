@@ -25,7 +25,7 @@ def attention(L, v, *, q=P, q_stride=256, max_pages=4, pool=8, sequences=1, rows
 
 def test_empty_calls_do_nothing(L):
     assert attention(L, view(), rows=0) == 0 and attention(L, view(), sequences=0) == 0
-    assert L.lcr_token_probs(None, 0, None, 0, 0, 5, None, None, None) == 0
+    assert L.lcr_token_probs(None, 0, None, 0, 0, 5, None, 0, None, None) == 0
     assert L.lcr_verify_drafts(None, None, None, 0, None, None, None, None, None, 0, 1, 5, None) == 0
     assert L.lcr_qk_norm_rope_kv(None, 0, None, 0, None, 0, 0, 1, None, None, 0.0, None, None, None, None) == 0
 
@@ -64,9 +64,11 @@ def test_plan_refuses(L):
 
 
 def test_probs_and_verify_refuse(L):
-    assert L.lcr_token_probs(P, 5, None, 5, 1, 5, None, None, None) == 1
-    assert L.lcr_token_probs(P, 4, P, 5, 1, 5, None, None, None) == 1
-    assert L.lcr_token_probs(P, 5, P, 5, 1, 0, None, None, None) == 1
+    assert L.lcr_token_probs(P, 5, None, 5, 1, 5, None, 0, None, None) == 1
+    assert L.lcr_token_probs(P, 4, P, 5, 1, 5, None, 0, None, None) == 1
+    assert L.lcr_token_probs(P, 5, P, 5, 1, 0, None, 0, None, None) == 1
+    assert L.lcr_token_probs(P, 5, P, 5, 2, 5, P, 1, None, None) == 1  # fewer temperatures than rows
+    assert L.lcr_token_probs(P, 5, P, 5, 2, 5, P, 0, P, None) == 1
     verify = lambda tokens=P, stride=9, k=2, vocab=9, drafts=P: L.lcr_verify_drafts(  # noqa: E731
         tokens, P, P, stride, P, drafts, P, None, P, 1, k, vocab, None)
     assert verify(tokens=None) == 1 and verify(stride=8) == 1 and verify(vocab=0) == 1 and verify(drafts=None) == 1

@@ -74,7 +74,7 @@ def run_plan(tables, held, stack, count, cached, new, done, ps, max_rows, alias)
                     free_count_out=co, row_starts=starts, kv_lengths=kv, positions=pos, slots=slots, row_sequence=seq)
     host = lambda x: x.cpu().numpy()  # noqa: E731
     rows = int(starts[-1])
-    assert (host(pos)[rows:] == -7).all() and (host(slots)[rows:] == -7).all()
+    assert (host(pos)[rows:] == 0).all() and (host(slots)[rows:] == -1).all() and (host(seq)[rows:] == -1).all()
     return dict(tables=host(t), held=host(ho), stack=host(s), count=int(co), starts=host(starts), kv=host(kv),
                 pos=host(pos)[:rows].tolist(), slots=host(slots)[:rows].tolist(), seq=host(seq)[:rows].tolist())
 
@@ -491,6 +491,8 @@ def test_token_probs_by_request_and_without_temperature():
     paged.token_probs(a, x, t, seq)
     paged.token_probs(b, x, t[seq.long()].contiguous())
     assert torch.equal(a, b)
+    paged.token_probs(b, x, t, i32([0, -1, 1, 2, 3, 2]))  # rows of no request
+    assert torch.equal(b[[0, 2, 3, 5]], a[[0, 2, 3, 5]]) and not b[[1, 4]].any()
     paged.token_probs(a, x)
     assert float((a.double() - torch.softmax(x.double(), 1)).abs().max()) < 1e-6
 
