@@ -5,8 +5,8 @@
 // Tiles. A tile is one KV head of one request and up to 128 of its (row, query
 // head) pairs: QB = 128 / G' rows (G' = the group rounded up to a power of
 // two) by the G heads of the group, pair r = row * G + head, so that a few
-// rows of a decoding request fill the lowest lanes. Keys come in blocks of
-// head_dim:
+// rows of a decoding request fill the lowest lanes. Keys come in blocks of as
+// many keys as a head has dimensions:
 //
 //   S = Q K^T          m128 k16, both from shared memory (K-major, 128-byte
 //                      swizzle), into TMEM
@@ -39,10 +39,30 @@
 // Loads. One warp fills a ring of 128-byte wide panels of K and V in the
 // swizzled layout, ahead across tiles. Where the pool is dense and a page holds
 // a multiple of 16 positions, by tensor copies of 16 to 128 keys; else 16 bytes
-// at a time (cp.async), each lane holding the cache rows of its keys: any page
-// size and strides, but the issue of a copy costs the warp about 15 cycles, and
-// it bounds the kernel (LOADS). Keys past the tile's last position are never
-// read and enter as zeros, so what lies there cannot reach the sums.
+// at a time (cp.async), each lane holding the cache rows of its keys, for any
+// page size and strides (the three cases below on pages of 16: 59, 42 and 801 us
+// by tensor copies, 61, 51 and 878 by cp.async). Keys past the tile's last
+// position are never read and enter as zeros, so what lies there cannot reach
+// the sums.
+//
+// What bounds it, measured on heads of 64, 32 query and 8 KV heads:
+//   64 requests of 1 - 5 rows on 128 - 4096 keys (279 MB of keys and values):
+//     59 us, 4.7 TB/s, 0.72 of a copy's rate. Memory, and 9 us of start (the
+//     scan, the first loads) and of joining split tiles.
+//   the same mix with a chunk of 509 rows: 42 us for 130 MB. The chain of a
+//     block, 4 - 5 thousand cycles with three other CTAs on the SM, ten blocks
+//     a CTA.
+//   2048 rows on 32768 keys: 801 us, 665 TFLOP/s. The chain again: 2900 cycles
+//     a block, of them 1500 in the softmax warps (shared with the other CTAs'),
+//     the rest the way to the tensor cores and back; tensor pipe 39 % and
+//     transcendental pipe 47 % busy, issue slots 55 %.
+//   2048 rows on 8192 keys, heads of 128: 274 us, 880 TFLOP/s. The keys and
+//     values that each tile of 128 pairs reads again, 6.7 TB/s out of L2.
+// Measured and no faster: P signalled in halves, so that P V starts early (812
+// us for the third case, 811 without); the last 32 scores kept in registers
+// between the two passes (809, spills); the next K waited for ahead of P (the
+// second case 48 us: P V, whose slots the loads need, came late); blocks of 128
+// keys with P beside S, for two CTAs an SM; two load warps for heads of 128.
 //
 // Warps: 0-3 softmax (warp w owns TMEM lanes 32 w .. + 31) and epilogue, 4
 // TMEM allocation and MMA issue, 5 loads. Every wait is bounded.
@@ -71,7 +91,8 @@ template <int BLK>
 constexpr int ca_min_range() {  // units of a range at least (where there are as many); at least ca_reach
   return ca_reach<BLK>();
 }
-constexpr int kCaFmaGroups = 1;   // of 8 pairs of exponentials, on the FMA pipe
+// Of 8 pairs of exponentials, on the FMA pipe (2048 rows on 32768 keys: 801 us, with none 814).
+constexpr int kCaFmaGroups = 1;
 
 struct ChunkAttnArgs {
   bf16* out;
@@ -760,17 +781,19 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
     do {
       const int cnt = w.count(), off = w.off(), key_end = w.key_end(a);
       if (cnt == 0) continue;
-      ok = wait(q_full, tile & 1);
-      for (int j = 0; j < cnt && ok; ++j, ++g) {
-        // K, then P V of the block before: S goes over its P.
-        const uint32_t k0 = slot;
+      auto panels = [&] {  // the next K's or V's first slot, once it has landed
+        const uint32_t first = slot;
 #pragma unroll
         for (int p = 0; p < G::PANELS; ++p) {
           ok = ok && wait(&full[slot], phase);
           step();
         }
+        return first;
+      };
+      // S goes over the P of the block before: its P V is waited for.
+      auto issue_s = [&](uint32_t k0) {
         if (g > 0) ok = ok && wait(pv_done, (g - 1) & 1);
-        if (!ok) break;
+        if (!ok) return;
         const uint64_t kdesc = tc_desc_sw128(ring_addr + k0 * G::SLOT);
         if (leader) {
 #pragma unroll
@@ -780,17 +803,18 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
               tc_mma(base, qdesc + p * (kCaRows * 128 / 16) + 2 * k, kdesc + p * (G::SLOT / 16) + 2 * k, idesc_s,
                      p + k > 0 ? 1u : 0u);
             }
-            tc_commit(&empty[k0 + p]);
           }
           tc_commit(s_full);
-        }
-        // V, then P.
-        const uint32_t v0 = slot;
 #pragma unroll
-        for (int p = 0; p < G::PANELS; ++p) {
-          ok = ok && wait(&full[slot], phase);
-          step();
+          for (int p = 0; p < G::PANELS; ++p) tc_commit(&empty[k0 + p]);
         }
+      };
+      ok = wait(q_full, tile & 1);
+      const uint32_t first = panels();
+      issue_s(first);
+      for (int j = 0; j < cnt && ok; ++j) {
+        const bool more = j + 1 < cnt;
+        const uint32_t v0 = panels();
         ok = ok && wait(p_full, g & 1);
         if (!ok) break;
         const uint64_t vdesc = ca_vdesc(ring_addr + v0 * G::SLOT, G::SLOT);
@@ -802,9 +826,16 @@ __global__ void __launch_bounds__(kCaThreads, CaGeom<D>::CTAS) chunk_attn_kernel
               tc_mma_ts(base + G::O_COL, base + k * 8u, vdesc + k * 2048 / 16, idesc_pv, j + k > 0 ? 1u : 0u);
             }
           }
+          tc_commit(pv_done);  // first what the chain waits for
 #pragma unroll
           for (int p = 0; p < G::PANELS; ++p) tc_commit(&empty[v0 + p]);
-          tc_commit(pv_done);
+        }
+        ++g;
+        if (more) {
+          // (Not before P V: the next K may come late, and its copies may need
+          // V's slots.)
+          const uint32_t k0 = panels();
+          issue_s(k0);
         }
       }
       ++tile;
