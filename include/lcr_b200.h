@@ -454,9 +454,10 @@ LCR_API int lcr_batch_time_steps(lcr_batch* batch, int steps, float* ms);
  * held and free_count themselves), row_starts [sequences + 1], kv_lengths
  * [sequences] (cached + new, 0 if refused), and for each row r < max_rows its
  * positions[r], slots[r] = page * page_size + position % page_size (-1 if
- * refused) and row_sequence[r] = b. Rows past max_rows are cut off; those
- * left over below it get 0, -1 and -1, so that a step captured in a graph for
- * max_rows rows runs with fewer.
+ * refused) and row_sequence[r] = b. Rows left over below max_rows get 0, -1
+ * and -1, so that a step captured in a graph for max_rows rows runs with
+ * fewer; rows past it are cut off (row_starts[sequences] is then max_rows, and
+ * the request that is cut must not go on to lcr_chunk_attention).
  * pool_pages * page_size must fit in 31 bits. */
 LCR_API int lcr_plan_step(int32_t* block_tables, int max_pages, const int32_t* held, int32_t* held_out,
                           int32_t* free_pages, const int32_t* free_count, int32_t* free_count_out,

@@ -40,24 +40,26 @@
 // swizzled layout, ahead across tiles. Where the pool is dense and a page holds
 // a multiple of 16 positions, by tensor copies of 16 to 128 keys; else 16 bytes
 // at a time (cp.async), each lane holding the cache rows of its keys, for any
-// page size and strides (the three cases below on pages of 16: 59, 42 and 801 us
-// by tensor copies, 61, 51 and 878 by cp.async). Keys past the tile's last
-// position are never read and enter as zeros, so what lies there cannot reach
-// the sums.
+// page size and strides (the first three cases below, on pages of 16: 59, 42
+// and 801 us by tensor copies, 61, 51 and 878 by cp.async). Keys past the tile's
+// last position are never read and enter as zeros, so what lies there cannot
+// reach the sums.
 //
-// What bounds it, measured on heads of 64, 32 query and 8 KV heads:
-//   64 requests of 1 - 5 rows on 128 - 4096 keys (279 MB of keys and values):
-//     59 us, 4.7 TB/s, 0.72 of a copy's rate. Memory, and 9 us of start (the
-//     scan, the first loads) and of joining split tiles.
-//   the same mix with a chunk of 509 rows: 42 us for 130 MB. The chain of a
-//     block, 4 - 5 thousand cycles with three other CTAs on the SM, ten blocks
-//     a CTA.
-//   2048 rows on 32768 keys: 801 us, 665 TFLOP/s. The chain again: 2900 cycles
-//     a block, of them 1500 in the softmax warps (shared with the other CTAs'),
-//     the rest the way to the tensor cores and back; tensor pipe 39 % and
-//     transcendental pipe 47 % busy, issue slots 55 %.
-//   2048 rows on 8192 keys, heads of 128: 274 us, 880 TFLOP/s. The keys and
+// What it measured, with 32 query and 8 KV heads, and what bounds it:
+//   64 requests of 1 - 5 rows on 128 - 4096 keys, heads of 64: 59 us for 279 MB
+//     of keys and values, 4.7 TB/s, 0.72 of a copy's rate. Memory, and 9 us of
+//     start (the scan, the first loads) and of joining split tiles.
+//   15 of these beside a chunk of 509 rows, heads of 128: 42 us for 130 MB, 0.47
+//     of a copy's rate. The chain of a block, 4 - 5 thousand cycles while loads
+//     come late, about ten blocks a CTA.
+//   2048 rows on 32768 keys, heads of 64: 801 us, 665 TFLOP/s, 0.39 of a large
+//     product's rate. The chain again: 2900 cycles a block, of them 1500 in the
+//     softmax warps (shared with the other CTAs'), the rest the way to the tensor
+//     cores and back; tensor cores 41 % and transcendental pipe 50 % busy, issue
+//     slots 57 %.
+//   2048 rows on 8192 keys, heads of 128: 266 us, 900 TFLOP/s. The keys and
 //     values that each tile of 128 pairs reads again, 6.7 TB/s out of L2.
+//   5 rows on 250 keys, heads of 64: 9.8 us, latency from end to end.
 // Measured and no faster: P signalled in halves, so that P V starts early (812
 // us for the third case, 811 without); the last 32 scores kept in registers
 // between the two passes (809, spills); the next K waited for ahead of P (the

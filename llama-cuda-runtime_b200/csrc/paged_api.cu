@@ -268,7 +268,8 @@ extern "C" int lcr_token_probs(float* probs, int64_t probs_stride, const float* 
                "token_probs: %d temperatures of %d rows", temperatures, rows);
   TokenProbsArgs a = {probs, probs_stride, logits, logits_stride, rows, vocab, temperature, temperatures, row_sequence, 0};
   // CTAs for a row: enough to keep it in shared memory, and for few rows as many
-  // as fill the GPU (one row of 128256 ids: 8 CTAs).
+  // as fill the GPU (one row of 32000 ids: 3.8 us with 8, 5.4 with the 2 it takes
+  // to keep it; 16 rows 4.9 and 5.6; 64 rows the same).
   int ctas = 1;
   while (ctas < kProbsMaxCtas && (vocab > ctas * kProbsSlice || (rows * ctas < 256 && vocab > ctas * 2048))) ctas *= 2;
   LCRB_REQUIRE(rows <= INT32_MAX / ctas, LCR_ERR_SHAPE, "token_probs: %d rows", rows);
@@ -291,7 +292,8 @@ extern "C" int lcr_verify_drafts(int32_t* tokens, int32_t* accepted, const float
                static_cast<long long>(target_stride), vocab);
   VerifyArgs a = {tokens,      accepted, target_probs, target_stride, target_starts, drafts, draft_counts,
                   draft_probs, uniforms, sequences,    max_drafts,    vocab};
-  // CTAs for a request: as many as run at once (two on an SM) for all of them.
+  // CTAs for a request: as many as run at once (two on an SM) for all of them
+  // (64 requests of 128256 ids: 41, 25, 19.5 and 23 us with 1, 2, 4 and 8).
   int ctas = 1;
   while (ctas < kVerifyMaxCtas && static_cast<long long>(sequences) * ctas * 2 <= 296) ctas *= 2;
   return launch_cluster(verify_drafts_kernel, sequences * ctas, ctas, kVerifyThreads, 0, cs(stream), a);

@@ -81,7 +81,9 @@ __device__ __forceinline__ int plan_add_rows(int x, int y, int most) {
 // and reading the tables back, so held and free_count may be updated in place.
 // A step of a few rows is bound by latency -- launch, the lengths' load, two
 // block barriers, a cluster barrier, the table's load -- and a large one by the
-// rows' stores, four rows a thread.
+// rows' stores, four rows a thread. 64 requests with up to five rows each: 7.1
+// us; 512 requests, 64 of them with chunks of up to 2048 rows: 21 us (one CTA
+// that did it all: 16.5 and 171 us, both timed with the call).
 __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) step_plan_kernel(const StepPlanArgs a) {
   extern __shared__ int32_t plan_smem[];
   int32_t* row_end = plan_smem;            // inclusive prefixes per request
