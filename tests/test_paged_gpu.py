@@ -648,6 +648,60 @@ def test_verify_drafts_keeps_the_target_distribution():
 # refusals
 # ---------------------------------------------------------------------------
 
+def test_a_captured_step_runs_with_fewer_rows():
+    """Plan, cache write, attention and probabilities in one graph of 12 rows:
+    replayed for steps of 12, 5 and 0 rows it gives what the entries give for
+    exactly those rows, and touches nothing else."""
+    g = torch.Generator(device=DEV).manual_seed(7)
+    heads, kvh, d, ps, pool, n, most = 4, 2, 64, 16, 24, 3, 12
+    inv = 10000.0 ** (-torch.arange(32, device=DEV) / 32.0)
+    qkv = torch.randn(most, (heads + 2 * kvh) * d, generator=g, device=DEV).bfloat16()
+    heat = torch.tensor([0.5, 1.0, 2.0], device=DEV)
+
+    def state():
+        rows = lambda: torch.full((most,), -7, dtype=torch.int32, device=DEV)  # noqa: E731
+        z = lambda *shape: torch.zeros(*shape, dtype=torch.bfloat16, device=DEV)  # noqa: E731
+        return dict(tables=torch.zeros(n, 8, dtype=torch.int32, device=DEV), held=i32([0] * n), stack=i32(range(pool)),
+                    count=i32([pool]), cached=i32([0] * n), new=i32([5, 1, 6]), starts=i32([0] * (n + 1)), kv=i32([0] * n),
+                    pos=rows(), slots=rows(), seq=rows(), keys=z(pool, kvh, ps, d), values=z(pool, kvh, ps, d),
+                    q=z(most, heads * d), out=torch.full((most, heads * d), 3.0, dtype=torch.bfloat16, device=DEV),
+                    probs=torch.full((most, d), 3.0, device=DEV), work=paged.attention_workspace(heads, d))
+
+    def step(s, rows):
+        pos, slots, seq = s["pos"][:rows], s["slots"][:rows], s["seq"][:rows]
+        paged.plan_step(s["tables"], s["held"], s["stack"], s["count"], s["cached"], s["new"], page_size=ps,
+                        held_out=s["held"], free_count_out=s["count"], row_starts=s["starts"], kv_lengths=s["kv"],
+                        positions=pos, slots=slots, row_sequence=seq)
+        paged.qk_norm_rope_kv(s["q"][:rows], s["keys"], s["values"], qkv[:rows], pos, slots, inv)
+        paged.chunk_attention(s["out"][:rows], s["q"][:rows], s["keys"], s["values"], s["tables"], s["starts"], s["kv"],
+                              scale=0.125, workspace=s["work"])
+        paged.token_probs(s["probs"][:rows], qkv[:rows, :d].float(), heat, seq)
+
+    a, b = state(), state()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step(a, most)
+    cached = np.zeros(n, int)
+    for new in ([5, 1, 6], [2, 0, 3], [0, 0, 0], [0, 12, 0]):
+        rows = sum(new)
+        for s in (a, b):
+            s["cached"].copy_(i32(cached))
+            s["new"].copy_(i32(new))
+            s["out"].fill_(3.0)
+        graph.replay()
+        step(b, rows)
+        paged.attention_status(a["work"])
+        for k in ("tables", "held", "stack", "count", "starts", "kv", "keys", "values"):
+            assert torch.equal(a[k], b[k]), (new, k)
+        for k in ("pos", "slots", "seq", "q", "out", "probs"):
+            assert torch.equal(a[k][:rows], b[k][:rows]), (new, k)
+        assert (a["out"][rows:] == 3.0).all() and not a["probs"][rows:].any()
+        assert (a["slots"][rows:] == -1).all() and (a["seq"][rows:] == -1).all()
+        cached += np.array(new)
+
+
 def test_refusals():
     c = attention_case([(2, 20)], 4, 2, 64, 16)
     out = torch.empty_like(c["q"])
