@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kProbsThreads, 3) token_probs_kernel(const Tok
   }
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-  const float k2 = kLog2e / t;
+  const float k2 = fminf(fmaxf(kLog2e / t, 2e-38f), 1e30f);  // 0 * inf, at the ends of t's range, is no weight
   const float base = m == -INFINITY ? 0.f : m;  // a slice of nothing but -inf weighs nothing
   float sum = 0.f;
 #pragma unroll 2

@@ -497,6 +497,18 @@ def test_token_probs_by_request_and_without_temperature():
     assert float((a.double() - torch.softmax(x.double(), 1)).abs().max()) < 1e-6
 
 
+def test_token_probs_at_the_ends_of_the_temperature():
+    """1e-40: everything on the largest logits; inf: the same on all that are
+    not -inf; NaN and below 0: the lowest of the largest."""
+    x = torch.tensor([[1.0, 3.0, -math.inf, 3.0, 2.0, -1e30, 0.0]], device=DEV).repeat(4, 1)
+    p = torch.empty_like(x)
+    paged.token_probs(p, x, torch.tensor([1e-40, math.inf, math.nan, -1.0], device=DEV))
+    want = torch.tensor([[0, 0.5, 0, 0.5, 0, 0, 0], [1 / 6, 1 / 6, 0, 1 / 6, 1 / 6, 1 / 6, 1 / 6],
+                         [0, 1, 0, 0, 0, 0, 0], [0, 1, 0, 0, 0, 0, 0]], device=DEV)
+    assert float((p[[0, 2, 3]] - want[[0, 2, 3]]).abs().max()) == 0
+    assert float((p[1] - want[1]).abs().max()) < 1e-6
+
+
 # ---------------------------------------------------------------------------
 # verify_drafts
 # ---------------------------------------------------------------------------
