@@ -37,6 +37,16 @@ int check_view(const char* what, const lcr_kv_view* v, int pool_pages) {
   return LCR_OK;
 }
 
+// Division of a number below 2^31 by the page size: with 2^s >= page_size, mul =
+// ceil(2^(31 + s) / page_size) is exact.
+void page_division(int page_size, unsigned* mul, unsigned* shift) {
+  int s = 0;
+  while ((1ll << s) < page_size) ++s;
+  if (s == 0) return;
+  *shift = static_cast<unsigned>(s - 1);
+  *mul = static_cast<unsigned>(((1ull << (31 + s)) + page_size - 1) / page_size);
+}
+
 // Of the current device.
 int multiprocessors() {
   int dev = 0, sms = 148;
@@ -116,10 +126,28 @@ extern "C" int lcr_plan_step(int32_t* block_tables, int max_pages, const int32_t
   LCRB_REQUIRE(static_cast<long long>(sequences) * max_pages <= INT32_MAX &&
                    static_cast<long long>(pool_pages) * page_size <= INT32_MAX,
                LCR_ERR_SHAPE, "plan_step: tables or pool pass 31 bits");
-  StepPlanArgs a = {block_tables, max_pages,  held,      held_out,   free_pages, free_count, free_count_out,
-                    pool_pages,   cached,     new_tokens, finished,   sequences,  page_size,  max_rows,
-                    row_starts,   kv_lengths, positions, slots,      row_sequence};
-  const size_t smem = sizeof(int32_t) * 4 * static_cast<size_t>(sequences);
+  StepPlanArgs a = {};
+  a.tables = block_tables;
+  a.max_pages = max_pages;
+  a.held = held;
+  a.held_out = held_out;
+  a.free_pages = free_pages;
+  a.free_count = free_count;
+  a.free_count_out = free_count_out;
+  a.pool_pages = pool_pages;
+  a.cached = cached;
+  a.new_tokens = new_tokens;
+  a.finished = finished;
+  a.sequences = sequences;
+  a.page_size = static_cast<uint32_t>(page_size);
+  page_division(page_size, &a.page_mul, &a.page_shift);
+  a.max_rows = max_rows;
+  a.row_starts = row_starts;
+  a.kv_lengths = kv_lengths;
+  a.positions = positions;
+  a.slots = slots;
+  a.row_sequence = row_sequence;
+  const size_t smem = sizeof(int32_t) * 5 * static_cast<size_t>(sequences);
   LCRB_CUDA(cudaFuncSetAttribute(step_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
   return launch_kernel(step_plan_kernel, dim3(kPlanCtas), dim3(kPlanThreads), smem, cs(stream), false, a);
 }
@@ -220,14 +248,7 @@ extern "C" int lcr_chunk_attention(void* out, int64_t out_stride, const void* q,
   a.scale_log2 = scale * kLog2e;
   a.log2_qb = 7;
   while (a.log2_qb > 0 && (a.group << a.log2_qb) > kCaRows) --a.log2_qb;
-  // Division by the page size: with 2^s >= page_size, mul = ceil(2^(31 + s) /
-  // page_size) is exact for keys below 2^31.
-  int s = 0;
-  while ((1ll << s) < view->page_size) ++s;
-  if (s > 0) {
-    a.page_shift = static_cast<unsigned>(s - 1);
-    a.page_mul = static_cast<unsigned>(((1ull << (31 + s)) + view->page_size - 1) / view->page_size);
-  }
+  page_division(view->page_size, &a.page_mul, &a.page_shift);
   const int ctas = attention_ctas(view->head_dim);
   char* work = static_cast<char*>(scratch);
   a.status = reinterpret_cast<uint32_t*>(work);

@@ -30,7 +30,10 @@ struct StepPlanArgs {
   const int32_t* cached;
   const int32_t* new_tokens;
   const int32_t* finished;
-  int sequences, page_size, max_rows;
+  int sequences;
+  uint32_t page_size;
+  unsigned page_mul, page_shift;  // position / page_size = umulhi(position, page_mul) >> page_shift (page_size > 1)
+  int max_rows;
   int32_t* row_starts;
   int32_t* kv_lengths;
   int32_t* positions;
@@ -52,8 +55,9 @@ __device__ __forceinline__ PlanNeed plan_need(const StepPlanArgs& a, int b) {
   const bool done = a.finished != nullptr && a.finished[b] != 0;
   r.back = done ? held : 0;
   r.held = done ? 0 : held;
-  const long long want = (static_cast<long long>(r.cached) + r.rows + a.page_size - 1) / a.page_size;
-  r.fits = want <= a.max_pages;
+  const uint32_t all = static_cast<uint32_t>(r.cached) + static_cast<uint32_t>(r.rows), q = all / a.page_size;
+  const uint32_t want = q + (all != q * a.page_size);
+  r.fits = want <= static_cast<uint32_t>(a.max_pages);
   r.need = r.fits ? max(0, static_cast<int>(want) - r.held) : 0;
   return r;
 }
@@ -81,15 +85,16 @@ __device__ __forceinline__ int plan_add_rows(int x, int y, int most) {
 // and reading the tables back, so held and free_count may be updated in place.
 // A step of a few rows is bound by latency -- launch, the lengths' load, two
 // block barriers, a cluster barrier, the table's load -- and a large one by the
-// rows' stores, four rows a thread. 64 requests with up to five rows each: 7.1
-// us; 512 requests, 64 of them with chunks of up to 2048 rows: 21 us (one CTA
+// rows' stores, four rows a thread. 64 requests with up to five rows each: 6.2
+// us; 512 requests, 64 of them with chunks of up to 2048 rows: 17.6 us (one CTA
 // that did it all: 16.5 and 171 us, both timed with the call).
 __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) step_plan_kernel(const StepPlanArgs a) {
   extern __shared__ int32_t plan_smem[];
   int32_t* row_end = plan_smem;            // inclusive prefixes per request
   int32_t* need_end = row_end + a.sequences;
   int32_t* back_end = need_end + a.sequences;
-  int32_t* base = back_end + a.sequences;  // pages held before this step's
+  int32_t* base = back_end + a.sequences;  // pages held before this step's; ~pages: the request does not fit its table
+  int32_t* cached = base + a.sequences;
   __shared__ int part[3][kPlanThreads / 32];
   __shared__ int used_s;
   const auto cluster = cooperative_groups::this_cluster();
@@ -111,7 +116,8 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     row_end[b] = rows;
     need_end[b] = need;
     back_end[b] = back;
-    base[b] = r.held;
+    base[b] = r.fits ? r.held : ~r.held;
+    cached[b] = r.cached;
   }
   auto scan = [&](int& x, int& y, int& z) {  // inclusive, over a warp
 #pragma unroll
@@ -182,20 +188,17 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     a.tables[static_cast<size_t>(b) * a.max_pages + base[b] + (k - first)] = __ldcg(a.free_pages + height - 1 - k);
   }
   cluster.sync();
-  auto granted = [&](int b, int c, int n) {
-    const long long want = (static_cast<long long>(c) + n + a.page_size - 1) / a.page_size;
-    const int nb = need_end[b] - (b > 0 ? need_end[b - 1] : 0);
-    return want <= a.max_pages && (nb == 0 || need_end[b] <= height);
+  auto granted = [&](int b) {
+    return base[b] >= 0 && (need_end[b] <= height || need_end[b] == (b > 0 ? need_end[b - 1] : 0));
   };
   // Per request, by one CTA (held may be held_out, free_count free_count_out:
   // every thread of the cluster has read them).
   if (cluster.block_rank() == 0) {
     for (int b = b0; b < b1; ++b) {
-      const int c = max(0, a.cached[b]), n = max(0, a.new_tokens[b]);
-      const bool got = granted(b, c, n);
+      const bool got = granted(b);
       a.row_starts[b] = b > 0 ? row_end[b - 1] : 0;
-      a.held_out[b] = base[b] + (got ? need_end[b] - (b > 0 ? need_end[b - 1] : 0) : 0);
-      a.kv_lengths[b] = got ? c + n : 0;
+      a.held_out[b] = base[b] < 0 ? ~base[b] : base[b] + (got ? need_end[b] - (b > 0 ? need_end[b - 1] : 0) : 0);
+      a.kv_lengths[b] = got ? cached[b] + max(0, a.new_tokens[b]) : 0;
     }
     if (tid == 0) {
       a.row_starts[B] = row_end[B - 1];
@@ -209,8 +212,8 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
   for (int r0 = 4 * me; r0 < total; r0 += 4 * kAll) {
     int b = plan_owner(row_end, B, r0);
     int begin = b > 0 ? row_end[b - 1] : 0, end = row_end[b];
-    int c = max(0, a.cached[b]), n = max(0, a.new_tokens[b]);
-    bool got = granted(b, c, n);
+    int c = cached[b];
+    bool got = granted(b);
     int pos[4], slot[4], seq[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -221,15 +224,14 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
             begin = end;
             end = row_end[++b];
           } while (r >= end);
-          c = max(0, a.cached[b]);
-          n = max(0, a.new_tokens[b]);
-          got = granted(b, c, n);
+          c = cached[b];
+          got = granted(b);
         }
         pos[e] = c + (r - begin);
         slot[e] = -1;
         seq[e] = b;
         if (got) {
-          const int q = pos[e] / a.page_size;
+          const int q = a.page_size == 1 ? pos[e] : static_cast<int>(__umulhi(pos[e], a.page_mul) >> a.page_shift);
           const int page = __ldcg(a.tables + static_cast<size_t>(b) * a.max_pages + q);
           if (page >= 0 && page < a.pool_pages) slot[e] = page * a.page_size + pos[e] - q * a.page_size;
         }
