@@ -85,8 +85,8 @@ __device__ __forceinline__ int plan_add_rows(int x, int y, int most) {
 // and reading the tables back, so held and free_count may be updated in place.
 // A step of a few rows is bound by latency -- launch, the lengths' load, two
 // block barriers, a cluster barrier, the table's load -- and a large one by the
-// rows' stores, four rows a thread. 64 requests with up to five rows each: 6.2
-// us; 512 requests, 64 of them with chunks of up to 2048 rows: 17.6 us (one CTA
+// rows' stores, four rows a thread. 64 requests with up to five rows each: 5.6
+// us; 512 requests, 64 of them with chunks of up to 2048 rows: 15.3 us (one CTA
 // that did it all: 16.5 and 171 us, both timed with the call).
 __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) step_plan_kernel(const StepPlanArgs a) {
   extern __shared__ int32_t plan_smem[];
@@ -214,10 +214,11 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     int begin = b > 0 ? row_end[b - 1] : 0, end = row_end[b];
     int c = cached[b];
     bool got = granted(b);
-    int pos[4], slot[4], seq[4];
+    int pos[4], slot[4], seq[4], at[4];  // at: the page's place in the tables, -1: none
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int r = r0 + e;
+      at[e] = -1;
       if (r < total) {
         if (r >= end) {
           do {
@@ -228,15 +229,18 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
           got = granted(b);
         }
         pos[e] = c + (r - begin);
-        slot[e] = -1;
         seq[e] = b;
-        if (got) {
-          const int q = a.page_size == 1 ? pos[e] : static_cast<int>(__umulhi(pos[e], a.page_mul) >> a.page_shift);
-          const int page = __ldcg(a.tables + static_cast<size_t>(b) * a.max_pages + q);
-          if (page >= 0 && page < a.pool_pages) slot[e] = page * a.page_size + pos[e] - q * a.page_size;
-        }
+        const int q = a.page_size == 1 ? pos[e] : static_cast<int>(__umulhi(pos[e], a.page_mul) >> a.page_shift);
+        slot[e] = pos[e] - q * a.page_size;
+        if (got) at[e] = b * a.max_pages + q;
       }
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (at[e] >= 0) at[e] = __ldcg(a.tables + at[e]);  // four loads at once
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) slot[e] = at[e] >= 0 && at[e] < a.pool_pages ? at[e] * static_cast<int>(a.page_size) + slot[e] : -1;
     if (wide && r0 + 4 <= total) {
       *reinterpret_cast<int4*>(a.positions + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
       *reinterpret_cast<int4*>(a.slots + r0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
