@@ -52,8 +52,8 @@
 //   15 of these beside a chunk of 509 rows, heads of 128: 42 us for 130 MB, 0.47
 //     of a copy's rate. The chain of a block, 4 - 5 thousand cycles while loads
 //     come late, about ten blocks a CTA.
-//   2048 rows on 32768 keys, heads of 64: 801 us, 665 TFLOP/s, 0.39 of a large
-//     product's rate. The chain again: 2900 cycles a block, of them 1500 in the
+//   2048 rows on 32768 keys, heads of 64: 801 us (790 - 815 between runs), 665
+//     TFLOP/s, 0.39 of a large product's rate. The chain again: 2900 cycles a block, of them 1500 in the
 //     softmax warps (shared with the other CTAs'), the rest the way to the tensor
 //     cores and back; tensor cores 41 % and transcendental pipe 50 % busy, issue
 //     slots 57 %.
