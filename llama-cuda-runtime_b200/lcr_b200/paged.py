@@ -80,12 +80,15 @@ def attention_workspace(heads: int, head_dim: int, device=None) -> torch.Tensor:
 def chunk_attention(out, q, keys, values, block_tables, row_starts, kv_lengths, *, scale: float,
                     workspace: Optional[torch.Tensor] = None) -> None:
     """Attention of each request's new rows (``q`` [rows, heads * head_dim],
-    packed) over its pages (``lcr_chunk_attention``)."""
+    packed) over its pages (``lcr_chunk_attention``). Without a ``workspace``
+    each stream keeps one of its own from its first call on."""
     operators = _lib or _operators()
     if workspace is None:
         key = (operators.current(), keys.shape[-1])
         workspace = _workspaces.get(key)
         if workspace is None:
+            if torch.cuda.is_current_stream_capturing():  # its memory would be the graph's
+                raise RuntimeError("chunk_attention: a stream's first call is captured; pass a workspace")
             workspace = _workspaces[key] = attention_workspace(q.shape[1] // keys.shape[-1], keys.shape[-1])
     status = operators.chunk_attention(out, q, keys, values, block_tables, row_starts, kv_lengths, scale, workspace)
     if status:

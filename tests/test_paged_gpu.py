@@ -394,6 +394,20 @@ def test_chunk_attention_in_a_graph():
     check_attention(c, out)
 
 
+def test_chunk_attention_keeps_no_workspace_of_a_graph():
+    """A stream whose first call is captured has to pass a workspace."""
+    c = attention_case([(2, 70)], 4, 2, 64, 16)
+    stream = torch.cuda.Stream()
+    kept = dict(paged._workspaces)
+    paged._workspaces.clear()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        with pytest.raises(RuntimeError, match="pass a workspace"):
+            run_attention(c)
+    assert not paged._workspaces
+    paged._workspaces.update(kept)
+
+
 def test_chunk_attention_page_outside_the_pool():
     """Reads as zeros and is reported once; the other requests are right."""
     c = attention_case([(2, 100), (3, 80)], 4, 2, 64, 16, seed=7, poison=False)
