@@ -12,7 +12,8 @@ them together.
 
 Every function writes into tensors of the caller, on torch's current stream,
 and allocates nothing (``chunk_attention`` keeps one workspace for each device
-and stream unless it is given one). Tensors must be on torch's current device;
+and stream unless it is given one, which a capture has to do). Tensors must be
+on torch's current device;
 what does not fit raises ``ValueError`` (``csrc/tensors.cpp`` checks them and calls
 the C ABI), what the library refuses ``runtime.LcrError``.
 """
@@ -81,14 +82,16 @@ def chunk_attention(out, q, keys, values, block_tables, row_starts, kv_lengths, 
                     workspace: Optional[torch.Tensor] = None) -> None:
     """Attention of each request's new rows (``q`` [rows, heads * head_dim],
     packed) over its pages (``lcr_chunk_attention``). Without a ``workspace``
-    each stream keeps one of its own from its first call on."""
+    each stream keeps one of its own from its first call on; a call in a
+    capture has to pass one, as the graph may be replayed beside calls on the
+    stream that it was captured on."""
     operators = _lib or _operators()
     if workspace is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("chunk_attention: a graph needs a workspace of its own; pass a workspace")
         key = (operators.current(), keys.shape[-1])
         workspace = _workspaces.get(key)
         if workspace is None:
-            if torch.cuda.is_current_stream_capturing():  # its memory would be the graph's
-                raise RuntimeError("chunk_attention: a stream's first call is captured; pass a workspace")
             workspace = _workspaces[key] = attention_workspace(q.shape[1] // keys.shape[-1], keys.shape[-1])
     status = operators.chunk_attention(out, q, keys, values, block_tables, row_starts, kv_lengths, scale, workspace)
     if status:

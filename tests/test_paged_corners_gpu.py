@@ -1,0 +1,35 @@
+"""Corners of the ragged step's operators (lcr_b200.paged): what a call among
+others, on odd values or with odd tensors, once got wrong or could."""
+import math
+import threading
+
+import numpy as np
+import pytest
+
+from lcr_b200 import runtime as rt
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():
+    pytest.skip("needs a CUDA device", allow_module_level=True)
+
+from lcr_b200 import paged  # noqa: E402
+from test_paged_gpu import DEV, attention_case, check_attention, i32, pools, run_attention, run_verify  # noqa: E402
+
+
+def test_chunk_attention_in_a_capture_needs_a_workspace():
+    """A graph may be replayed on any stream, beside calls on the one it was
+    captured on: what a stream keeps must not get into it."""
+    c = attention_case([(2, 70)], 4, 2, 64, 16)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        first = run_attention(c)  # the stream keeps a workspace from here on
+    out = torch.empty_like(first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        with pytest.raises(RuntimeError, match="pass a workspace"):
+            paged.chunk_attention(out, c["q"], c["keys"], c["values"], c["tables"], c["starts"], c["kv"], scale=0.125)
+    with torch.cuda.stream(stream):
+        assert torch.equal(run_attention(c), first)
