@@ -132,6 +132,9 @@ class Speculator:
         self.steps = 0
 
     def run(self, requests: List[Request]) -> None:
+        for i, r in enumerate(requests):
+            if not r.prompt:
+                raise ValueError(f"request {i} has an empty prompt")
         waiting = list(requests)
         while waiting or any(self.slots):
             for i, r in enumerate(self.slots):

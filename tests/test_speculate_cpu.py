@@ -1,0 +1,78 @@
+"""The host side of lcr_b200.speculate over a model of plain Python: which rows
+a step brings, and what is refused."""
+import types
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from lcr_b200 import paged, speculate as sp  # noqa: E402
+
+VOCAB = 31
+
+
+class Rows:
+    """Stands for RaggedModel: the next token after t at position p is
+    (t + p + 1) % VOCAB. A row is (request, position, token)."""
+
+    def __init__(self, slots=2, max_seq=48, page_size=16):
+        self.w = types.SimpleNamespace(device=torch.device("cpu"))
+        self.slots, self.page_size = slots, page_size
+        self.tables = torch.zeros(slots, -(-max_seq // page_size), dtype=torch.int32)
+        self.kv_lengths = torch.zeros(slots, dtype=torch.int32)
+        self.steps = []
+
+    def forward(self, tokens, cached, new_tokens, finished, wanted):
+        rows = []
+        for b, (c, n) in enumerate(zip(cached.tolist(), new_tokens.tolist())):
+            for i in range(n):
+                rows.append((b, c + i, int(tokens[len(rows)])))
+        assert len(rows) == tokens.numel() and all(0 <= w < len(rows) for w in wanted.tolist())
+        self.kv_lengths = cached + new_tokens
+        self.steps.append(rows)
+        logits = torch.zeros(wanted.numel(), VOCAB)
+        for i, w in enumerate(wanted.tolist()):
+            logits[i, (rows[w][2] + rows[w][1] + 1) % VOCAB] = 1.0
+        return logits
+
+
+def greedy(prompt, n):
+    t = list(prompt)
+    for _ in range(n):
+        t.append((t[-1] + len(t)) % VOCAB)
+    return t[len(prompt):]
+
+
+@pytest.fixture(autouse=True)
+def plain_operators(monkeypatch):
+    def verify(tokens, accepted, probs, starts, drafts, counts, draft_probs, uniforms):
+        tokens.fill_(-1)
+        accepted.zero_()
+        for b in range(drafts.shape[0]):
+            if starts[b + 1] > starts[b]:
+                best = probs[starts[b + 1] - 1 - counts[b]:starts[b + 1]].argmax(1)
+                while accepted[b] < counts[b] and drafts[b, accepted[b]] == best[accepted[b]]:
+                    accepted[b] += 1
+                tokens[b, :accepted[b] + 1] = best[:accepted[b] + 1]
+
+    monkeypatch.setattr(paged, "token_probs", lambda *a: None)
+    monkeypatch.setattr(paged, "verify_drafts", verify)
+
+
+@pytest.mark.parametrize("drafts", [0, 3])
+def test_tokens_of_requests(drafts):
+    model = Rows()
+    requests = [sp.Request(list(range(p)), n) for p, n in ((1, 9), (20, 5), (7, 12), (40, 9))]
+    sp.Speculator(model, drafts=drafts, chunk=8).run(requests)
+    for r in requests:
+        assert r.generated == greedy(r.prompt, r.new_tokens)
+
+
+def test_an_empty_prompt_is_refused():
+    """It has no last token to continue: nothing of the call runs, and the
+    requests beside it stay as they were."""
+    for requests in ([sp.Request([], 4)], [sp.Request([1, 2], 4), sp.Request([], 4)]):
+        model = Rows()
+        with pytest.raises(ValueError, match="request .*prompt"):
+            sp.Speculator(model).run(requests)
+        assert not model.steps and not requests[0].tokens
