@@ -135,6 +135,10 @@ class Speculator:
         for i, r in enumerate(requests):
             if not r.prompt:
                 raise ValueError(f"request {i} has an empty prompt")
+            # (The last token needs no place in the cache.)
+            longest, holds = len(r.prompt) + max(1, r.new_tokens) - 1, self.model.tables.shape[1] * self.model.page_size
+            if longest > holds:
+                raise ValueError(f"request {i} has up to {longest} positions; a slot's table holds {holds}")
         waiting = list(requests)
         while waiting or any(self.slots):
             for i, r in enumerate(self.slots):

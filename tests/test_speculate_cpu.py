@@ -76,3 +76,12 @@ def test_an_empty_prompt_is_refused():
         with pytest.raises(ValueError, match="request .*prompt"):
             sp.Speculator(model).run(requests)
         assert not model.steps and not requests[0].tokens
+
+
+def test_a_request_longer_than_its_table_is_refused():
+    """The last token needs no place in the cache: 48 positions hold 40 and 9."""
+    sp.Speculator(Rows()).run([sp.Request([3] * 40, 9)])
+    model = Rows()
+    with pytest.raises(ValueError, match="request 1 .*49 positions.*48"):
+        sp.Speculator(model).run([sp.Request([1], 2), sp.Request([3] * 40, 10)])
+    assert not model.steps
