@@ -143,8 +143,8 @@ class Speculator:
         while waiting or any(self.slots):
             for i, r in enumerate(self.slots):
                 if r is None and waiting:
-                    self.slots[i] = waiting.pop(0)
-                    self.slots[i].tokens = list(self.slots[i].prompt)
+                    r = self.slots[i] = waiting.pop(0)
+                    r.tokens, r.cached, r.drafted, r.accepted = list(r.prompt), 0, 0, 0
             self.step()
 
     def step(self) -> None:

@@ -85,3 +85,10 @@ def test_a_request_longer_than_its_table_is_refused():
     with pytest.raises(ValueError, match="request 1 .*49 positions.*48"):
         sp.Speculator(model).run([sp.Request([1], 2), sp.Request([3] * 40, 10)])
     assert not model.steps
+
+
+def test_a_request_runs_again():
+    r = sp.Request([5, 6, 7, 5, 6], 6)
+    for drafts in (4, 0):
+        sp.Speculator(Rows(), drafts=drafts).run([r])
+        assert r.generated == greedy([5, 6, 7, 5, 6], 6) and (r.drafted == 0) == (drafts == 0)
