@@ -133,7 +133,7 @@ class Speculator:
 
     def run(self, requests: List[Request]) -> None:
         for i, r in enumerate(requests):
-            if not r.prompt:
+            if len(r.prompt) == 0:
                 raise ValueError(f"request {i} has an empty prompt")
             # (The last token needs no place in the cache.)
             longest, holds = len(r.prompt) + max(1, r.new_tokens) - 1, self.model.tables.shape[1] * self.model.page_size

@@ -92,3 +92,10 @@ def test_a_request_runs_again():
     for drafts in (4, 0):
         sp.Speculator(Rows(), drafts=drafts).run([r])
         assert r.generated == greedy([5, 6, 7, 5, 6], 6) and (r.drafted == 0) == (drafts == 0)
+
+
+def test_a_prompt_may_be_an_array():
+    numpy = pytest.importorskip("numpy")
+    r = sp.Request(numpy.arange(1, 6), 3)
+    sp.Speculator(Rows()).run([r])
+    assert r.generated == greedy([1, 2, 3, 4, 5], 3)
