@@ -52,9 +52,9 @@ __device__ __forceinline__ bool probs_temperature(const TokenProbsArgs& a, int r
   return true;
 }
 
-// The order of (logit, lowest id first) as an integer.
+// The order of (logit, lowest id first) as an integer. x + 0.0f: -0.0 equals 0.0.
 __device__ __forceinline__ unsigned long long probs_key(float x, int i) {
-  const uint32_t b = __float_as_uint(x), k = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  const uint32_t b = __float_as_uint(__fadd_rn(x, 0.0f)), k = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
   return (static_cast<unsigned long long>(k) << 32) | (0xffffffffu - static_cast<uint32_t>(i));
 }
 

@@ -33,3 +33,17 @@ def test_chunk_attention_in_a_capture_needs_a_workspace():
             paged.chunk_attention(out, c["q"], c["keys"], c["values"], c["tables"], c["starts"], c["kv"], scale=0.125)
     with torch.cuda.stream(stream):
         assert torch.equal(run_attention(c), first)
+
+
+@pytest.mark.parametrize("vocab", [3, 999, 128256])
+def test_token_probs_zeros_of_either_sign_tie(vocab):
+    """Greedy: -0.0 and 0.0 are equal, so the lower id of them is taken."""
+    x = torch.full((3, vocab), -1.0, device=DEV)
+    x[0, 0], x[0, vocab - 1] = -0.0, 0.0
+    x[1, 0], x[1, vocab - 1] = 0.0, -0.0
+    x[2, 1], x[2, vocab - 1] = -0.0, -0.0
+    p = torch.empty_like(x)
+    paged.token_probs(p, x, torch.zeros(3, device=DEV))
+    want = torch.zeros_like(x)
+    want[[0, 1, 2], [0, 0, 1]] = 1.0
+    assert torch.equal(p, want)
