@@ -512,9 +512,10 @@ LCR_API int lcr_chunk_attention_status(void* scratch, lcr_stream_t stream);
 /* Rows of fp32 logits to probabilities: probs = softmax(logits / t) with t =
  * temperature[row_sequence[r]] (row_sequence NULL: temperature[r];
  * temperature NULL: 1), of which there are temperatures; t <= 0 puts
- * everything on the largest logit (lowest id on ties). Logits of -inf get 0;
- * a row of nothing but -inf, or of a request outside the temperatures (-1), is
- * all zeros. probs may be logits itself. Row strides in elements. */
+ * everything on the largest logit (lowest id on ties, zeros of either sign
+ * alike; a NaN is passed over). Logits of -inf get 0; a row of nothing but
+ * -inf, or of a request outside the temperatures (-1), is all zeros; with t >
+ * 0 a NaN among the logits makes the row NaN. probs may be logits itself. Row strides in elements. */
 LCR_API int lcr_token_probs(float* probs, int64_t probs_stride, const float* logits, int64_t logits_stride,
                             int rows, int vocab, const float* temperature, int temperatures,
                             const int32_t* row_sequence, lcr_stream_t stream);

@@ -182,10 +182,11 @@ __global__ void __launch_bounds__(kProbsThreads, 3) token_probs_kernel(const Tok
   for (int q = lane; q < ctas * kProbsWarps; q += 32) top = fmaxf(top, ms[q].x);
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  for (int q = lane; q < ctas * kProbsWarps; q += 32) all += ms[q].x == -INFINITY ? 0.f : ms[q].y * exp2f((ms[q].x - top) * k2);
+  for (int q = lane; q < ctas * kProbsWarps; q += 32) all += ms[q].y * (ms[q].x == -INFINITY ? 0.f : exp2f((ms[q].x - top) * k2));
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
-  const float f = m == -INFINITY ? 0.f : exp2f((m - top) * k2) / all;
+  // (A NaN logit has made its warp's sum NaN, and with it the row.)
+  const float f = m == -INFINITY ? 0.f * all : exp2f((m - top) * k2) / all;
 #pragma unroll 2
   for (int k = 0; k < groups; ++k) {
     const float4 q = mine[k * kProbsThreads];

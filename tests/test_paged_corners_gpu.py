@@ -47,3 +47,20 @@ def test_token_probs_zeros_of_either_sign_tie(vocab):
     want = torch.zeros_like(x)
     want[[0, 1, 2], [0, 0, 1]] = 1.0
     assert torch.equal(p, want)
+
+
+@pytest.mark.parametrize("vocab", [4, 5000, 128256, 300007])
+def test_token_probs_of_a_row_with_nan(vocab):
+    """A NaN among the logits makes the whole row NaN, as in the formula, also
+    where its neighbours are -inf; rows beside it are untouched."""
+    x = torch.randn(3, vocab, generator=torch.Generator(device=DEV).manual_seed(vocab), device=DEV)
+    x[1, :vocab // 2] = -math.inf
+    x[1, 1] = math.nan
+    p = torch.empty_like(x)
+    paged.token_probs(p, x, torch.ones(3, device=DEV))
+    assert bool(p[1].isnan().all())
+    q = torch.empty_like(x[:1])
+    for r in (0, 2):
+        paged.token_probs(q, x[r:r + 1], torch.ones(1, device=DEV))
+        # (A single row may go to another number of blocks: sums in another order.)
+        assert float((q[0] - p[r]).abs().max()) <= 1e-6 * float(q.max())
