@@ -11,6 +11,7 @@
 #include <dlfcn.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <string>
 
 #include "lcr_b200.h"
@@ -70,9 +71,24 @@ class Call {
     }
     return static_cast<T*>(t.data_ptr());
   }
+  bool absent(int i) const { return args_[i] == Py_None; }
   template <class T>
   T* maybe(int i, const char* name, at::ScalarType type, int64_t n) {
-    return args_[i] == Py_None ? nullptr : flat<T>(i, name, type, n);
+    return absent(i) ? nullptr : flat<T>(i, name, type, n);
+  }
+  // Contiguous, at least n elements, and `steps` (the elements from one index to
+  // the next of the layout that is read) has those of its own dimensions: a
+  // padded or a transposed one would be misread.
+  template <class T>
+  T* dense(int i, const char* name, at::ScalarType type, int64_t n, at::IntArrayRef steps, const char* wanted) {
+    T* p = flat<T>(i, name, type, n);
+    const at::Tensor& t = THPVariable_Unpack(args_[i]);
+    int64_t step = 1;
+    for (int64_t d = t.dim() - 1; d > 0; --d) {
+      step *= t.size(d);
+      if (step != 1 && std::find(steps.begin(), steps.end(), step) == steps.end()) refuse(i, name, wanted);
+    }
+    return p;
   }
   int64_t numel(int i) { return THPVariable_Unpack(args_[i]).numel(); }
   int32_t* ints(int i, const char* name, int64_t n) { return flat<int32_t>(i, name, at::kInt, n); }
@@ -211,11 +227,14 @@ int verify_drafts(PyObject* const* args, Py_ssize_t nargs) {
   const at::Tensor& p = c.rows(2, "target_probs", at::kFloat);
   const int n = c.small(d.size(0)), k = c.small(d.size(1)), vocab = c.small(p.size(1));
   Call::fits(t.size(0) == n && t.size(1) == k + 1, "tokens: [requests, max_drafts + 1]");
-  const int64_t cells = static_cast<int64_t>(n) * (k + 1);
+  const int64_t most = k, ids = vocab;
+  float* q = c.absent(6) ? nullptr
+                         : c.dense<float>(6, "draft_probs", at::kFloat, n * most * ids, {ids, most * ids},
+                                          "contiguous Float [requests, max_drafts, vocab]");
+  float* u = c.dense<float>(7, "uniforms", at::kFloat, n * (most + 1), {most + 1}, "contiguous Float [requests, max_drafts + 1]");
   return verify_drafts_c(static_cast<int32_t*>(t.data_ptr()), c.ints(1, "accepted", n), static_cast<const float*>(p.data_ptr()),
                          p.stride(0), c.ints(3, "target_starts", n + 1), c.ints(4, "drafts", 0), c.ints(5, "draft_counts", n),
-                         c.maybe<float>(6, "draft_probs", at::kFloat, static_cast<int64_t>(n) * k * vocab),
-                         c.flat<float>(7, "uniforms", at::kFloat, cells), n, k, vocab, c.stream());
+                         q, u, n, k, vocab, c.stream());
 }
 
 template <int (*F)(PyObject* const*, Py_ssize_t)>

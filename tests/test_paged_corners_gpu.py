@@ -64,3 +64,31 @@ def test_token_probs_of_a_row_with_nan(vocab):
         paged.token_probs(q, x[r:r + 1], torch.ones(1, device=DEV))
         # (A single row may go to another number of blocks: sums in another order.)
         assert float((q[0] - p[r]).abs().max()) <= 1e-6 * float(q.max())
+
+
+def test_verify_drafts_refuses_other_layouts():
+    """draft_probs and uniforms are read densely as [requests][max_drafts]
+    [vocab] and [requests][max_drafts + 1]: padded or transposed ones would be
+    misread. Room for more requests, and flat buffers, are as good."""
+    n, k, v = 3, 2, 10
+    g = torch.Generator(device=DEV).manual_seed(8)
+    p, q = (torch.softmax(torch.randn(m, v, generator=g, device=DEV), 1) for m in (n * (k + 1), n * k))
+    u = torch.rand(n, k + 1, generator=g, device=DEV)
+    args = dict(target_probs=p, target_starts=i32([0, 3, 6, 9]), drafts=i32(np.ones((n, k))), draft_counts=i32([2, 1, 0]),
+                draft_probs=q.view(n, k, v), uniforms=u)
+
+    def run(**kw):
+        tokens, accepted = i32(np.zeros((n, k + 1))), i32(np.zeros(n))
+        paged.verify_drafts(tokens, accepted, **{**args, **kw})
+        return tokens
+
+    want = run()
+    for kw in [dict(draft_probs=q), dict(draft_probs=q.view(n, k * v)), dict(draft_probs=q.flatten()),
+               dict(draft_probs=torch.cat((q, q)).view(2 * n, k, v)), dict(uniforms=u.flatten()),
+               dict(uniforms=torch.cat((u, u))), dict(uniforms=u[..., None])]:
+        assert torch.equal(run(**kw), want)
+    for name, shape in [("draft_probs", (n, k, v + 2)), ("draft_probs", (n, k + 1, v)), ("draft_probs", (n, v, k)),
+                        ("draft_probs", (n * k, v + 1)), ("draft_probs", (n, k, v - 1)), ("uniforms", (n, k + 2)),
+                        ("uniforms", (k + 1, n + 1)), ("uniforms", (n - 1, k + 1))]:
+        with pytest.raises(ValueError, match=name):
+            run(**{name: torch.full(shape, 0.5, device=DEV)})
