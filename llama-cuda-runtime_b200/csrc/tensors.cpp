@@ -90,6 +90,12 @@ class Call {
     }
     return p;
   }
+  // The gain of a norm, for the elements of one head (of every head the same).
+  void* gain(int i, const char* name, int64_t d) {
+    void* p = maybe<void>(i, name, at::kBFloat16, d);
+    if (p != nullptr && numel(i) != d) refuse(i, name, std::to_string(d) + " elements, for every head the same");
+    return p;
+  }
   int64_t numel(int i) { return THPVariable_Unpack(args_[i]).numel(); }
   int32_t* ints(int i, const char* name, int64_t n) { return flat<int32_t>(i, name, at::kInt, n); }
   // Rows of dense elements.
@@ -181,7 +187,7 @@ int qk_norm_rope_kv(PyObject* const* args, Py_ssize_t nargs) {
   Call::fits(heads > 0 && x.size(1) == (heads + 2 * view.num_kv_heads) * d && q.size(0) == rows && q.size(1) == heads * d,
              "qkv and q_out do not fit the pools' heads");
   return qk_norm_rope_kv_c(q.data_ptr(), q.stride(0), &view, pages, x.data_ptr(), x.stride(0), rows, c.small(heads),
-                           c.maybe<void>(7, "q_gain", at::kBFloat16, d), c.maybe<void>(8, "k_gain", at::kBFloat16, d),
+                           c.gain(7, "q_gain", d), c.gain(8, "k_gain", d),
                            static_cast<float>(c.number(9)), c.flat<float>(6, "inv_freq", at::kFloat, d / 2),
                            c.ints(4, "positions", rows), c.ints(5, "slots", rows), c.stream());
 }

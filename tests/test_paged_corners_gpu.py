@@ -92,3 +92,17 @@ def test_verify_drafts_refuses_other_layouts():
                         ("uniforms", (k + 1, n + 1)), ("uniforms", (n - 1, k + 1))]:
         with pytest.raises(ValueError, match=name):
             run(**{name: torch.full(shape, 0.5, device=DEV)})
+
+
+def test_qk_norm_rope_kv_refuses_gains_of_several_heads():
+    """Gains are one per element of a head, the same for all heads: a gain for
+    each head is not taken in part."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    keys, values = pools(2, 2, 16, 64, g)
+    qkv = torch.randn(2, 8 * 64, generator=g, device=DEV).bfloat16()
+    q, at = torch.empty(2, 4 * 64, dtype=torch.bfloat16, device=DEV), i32([0, 1])
+    inv, gain = torch.ones(32, device=DEV), torch.ones(64, dtype=torch.bfloat16, device=DEV)
+    paged.qk_norm_rope_kv(q, keys, values, qkv, at, at, inv, gain, gain[None])
+    for bad in [dict(q_gain=gain.repeat(4)), dict(k_gain=gain.repeat(2).view(2, 64)), dict(k_gain=gain[:32])]:
+        with pytest.raises(ValueError, match=next(iter(bad))):
+            paged.qk_norm_rope_kv(q, keys, values, qkv, at, at, inv, **{**dict(q_gain=gain, k_gain=gain), **bad})
