@@ -472,7 +472,8 @@ LCR_API int lcr_plan_step(int32_t* block_tables, int max_pages, const int32_t* h
  * elements. Each q and k head x becomes x * rsqrt(mean(x^2) + eps) * gain
  * (q_gain / k_gain [head_dim] bf16; NULL = no norm), then is rotated
  * (rotate-half, angle = positions[r] * inv_freq[i], i < head_dim / 2) -- all
- * in fp32, rounded to bf16 once. q goes to q_out (row stride q_stride), k and
+ * in fp32, rounded to bf16 once; the angles' cosines and sines are within 1e-5
+ * up to angles of 2^20. q goes to q_out (row stride q_stride), k and
  * v to slot slots[r] of the pools (page slots[r] / page_size); a row whose
  * slot is outside the pool (-1) writes no K / V. Rows of one call must have
  * distinct slots. q_out may be qkv itself (with q_stride = qkv_stride).

@@ -6,10 +6,11 @@
 //   out[i]       = y[i] cos t - y[i + D/2] sin t
 //   out[i + D/2] = y[i + D/2] cos t + y[i] sin t
 // in fp32, rounded to bf16 once. The angle is formed as a rounded product
-// plus its error (one fma), and the pair (cos, sin) is turned by that error
-// to first order: at position 32768 the plain fp32 product is off by up to
-// 2e-3, which would show in bf16; the second-order rest is below 1e-5 up to
-// position 10^6.
+// plus its error e (one fma), and the pair (cos, sin) is turned by that error
+// to second order: at position 32768 the plain fp32 product is off by up to
+// 1e-3, which would show in bf16, and at 2^20 by 2^-5. The rest, e^3 / 6, is
+// below 1e-5 up to angles of 2^20 (the first order alone: 5e-4 there); positions
+// are whole in fp32 up to 2^24.
 #pragma once
 
 #include "common.cuh"
@@ -40,7 +41,8 @@ __device__ __forceinline__ float2 rope_pair(int position, float inv_freq) {
   const float err = fmaf(p, inv_freq, -t);
   float s, c;
   sincosf(t, &s, &c);
-  return make_float2(fmaf(-err, s, c), fmaf(err, c, s));
+  const float half = -0.5f * err * err;
+  return make_float2(fmaf(half, c, fmaf(-err, s, c)), fmaf(half, s, fmaf(err, c, s)));
 }
 
 // Two bf16 in one conversion.

@@ -106,3 +106,25 @@ def test_qk_norm_rope_kv_refuses_gains_of_several_heads():
     for bad in [dict(q_gain=gain.repeat(4)), dict(k_gain=gain.repeat(2).view(2, 64)), dict(k_gain=gain[:32])]:
         with pytest.raises(ValueError, match=next(iter(bad))):
             paged.qk_norm_rope_kv(q, keys, values, qkv, at, at, inv, **{**dict(q_gain=gain, k_gain=gain), **bad})
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_qk_norm_rope_kv_far_positions(d):
+    """Positions up to 2^20. One rounding to bf16 (2^-8 of the value); the
+    turn's pair is off by 1e-5 at most there, on two terms."""
+    g = torch.Generator(device=DEV).manual_seed(d)
+    rows, heads, kvh = 512, 6, 2
+    keys, values = pools(rows // 16, kvh, 16, d, g)
+    qkv = torch.randn(rows, (heads + 2 * kvh) * d, generator=g, device=DEV).bfloat16()
+    pos = torch.randint(2 ** 17, 2 ** 20, (rows,), generator=g, device=DEV).to(torch.int32)
+    pos[0] = 2 ** 20 - 1
+    inv = (500000.0 ** (-torch.arange(0, d, 2, dtype=torch.float64) / d)).float().to(DEV)
+    q = torch.empty(rows, heads * d, dtype=torch.bfloat16, device=DEV)
+    paged.qk_norm_rope_kv(q, keys, values, qkv, pos, torch.arange(rows, dtype=torch.int32, device=DEV), inv)
+    x = qkv.double().view(rows, -1, d)[:, :heads + kvh]
+    a = pos.double()[:, None, None] * inv.double()
+    lo, hi = x[..., :d // 2], x[..., d // 2:]
+    want = torch.cat((lo * a.cos() - hi * a.sin(), hi * a.cos() + lo * a.sin()), -1)
+    k = keys.permute(0, 2, 1, 3).reshape(rows, kvh, d)
+    got = torch.cat((q.view(rows, heads, d), k), 1).double()
+    assert bool(((got - want).abs() <= want.abs() * 2.0 ** -8 + 2e-5 * float(want.abs().max())).all())
