@@ -147,8 +147,12 @@ extern "C" int lcr_plan_step(int32_t* block_tables, int max_pages, const int32_t
   a.positions = positions;
   a.slots = slots;
   a.row_sequence = row_sequence;
-  const size_t smem = sizeof(int32_t) * 5 * static_cast<size_t>(sequences);
-  LCRB_CUDA(cudaFuncSetAttribute(step_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  // The limit is the kernel's, not the launch's: always the largest call's, as
+  // other threads may be planning.
+  constexpr int kPerSequence = 5 * sizeof(int32_t);
+  const size_t smem = kPerSequence * static_cast<size_t>(sequences);
+  LCRB_CUDA(cudaFuncSetAttribute(step_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kPerSequence * LCR_PLAN_MAX_SEQUENCES));
   return launch_kernel(step_plan_kernel, dim3(kPlanCtas), dim3(kPlanThreads), smem, cs(stream), false, a);
 }
 

@@ -128,3 +128,29 @@ def test_qk_norm_rope_kv_far_positions(d):
     k = keys.permute(0, 2, 1, 3).reshape(rows, kvh, d)
     got = torch.cat((q.view(rows, heads, d), k), 1).double()
     assert bool(((got - want).abs() <= want.abs() * 2.0 ** -8 + 2e-5 * float(want.abs().max())).all())
+
+
+def test_plan_step_from_several_threads():
+    """Host threads plan steps of different sizes at the same time."""
+    L = rt.lib()
+    bad = {}
+
+    def go(n):
+        ints = lambda k: torch.zeros(k, dtype=torch.int32, device=DEV)  # noqa: E731
+        t, h, s, c, cached, new, starts, kv, row = (ints(k) for k in (n, n, 4, 1, n, n, n + 1, n, 4))
+        ptr = [x.data_ptr() for x in (t, h, s, c, cached, new, starts, kv, row)]
+        t, h, s, c, cached, new, starts, kv, row = ptr
+        torch.cuda.synchronize()
+        start.wait()
+        bad[n] = sum(L.lcr_plan_step(t, 1, h, h, s, c, c, 4, cached, new, None, n, 16, 4, starts, kv, row, row, row,
+                                     None) != 0 for _ in range(4000))
+        torch.cuda.synchronize()
+
+    sizes = [8192, 1, 64, 3000]
+    start = threading.Barrier(len(sizes))
+    threads = [threading.Thread(target=go, args=(n,)) for n in sizes]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert bad == {n: 0 for n in sizes}
