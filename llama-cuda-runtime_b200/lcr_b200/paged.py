@@ -89,10 +89,14 @@ def chunk_attention(out, q, keys, values, block_tables, row_starts, kv_lengths, 
     if workspace is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("chunk_attention: a graph needs a workspace of its own; pass a workspace")
-        key = (operators.current(), keys.shape[-1])
+        head_dim = keys.shape[-1] if isinstance(keys, torch.Tensor) and keys.dim() == 4 else 0
+        key = (operators.current(), head_dim)
         workspace = _workspaces.get(key)
         if workspace is None:
-            workspace = _workspaces[key] = attention_workspace(q.shape[1] // keys.shape[-1], keys.shape[-1])
+            if head_dim in (64, 128):  # (whatever the number of heads)
+                workspace = _workspaces[key] = attention_workspace(1, head_dim)
+            else:  # refused below
+                workspace = torch.empty(16, dtype=torch.uint8, device=torch.cuda.current_device())
     status = operators.chunk_attention(out, q, keys, values, block_tables, row_starts, kv_lengths, scale, workspace)
     if status:
         rt.check(status)

@@ -154,3 +154,20 @@ def test_plan_step_from_several_threads():
     for t in threads:
         t.join()
     assert bad == {n: 0 for n in sizes}
+
+
+def test_chunk_attention_checks_before_it_keeps_a_workspace():
+    c = attention_case([(2, 20)], 4, 2, 64, 16)
+    wide = torch.zeros(2, 2, 16, 96, dtype=torch.bfloat16, device=DEV)
+    out = torch.empty_like(c["q"])
+    rest = (c["tables"], c["starts"], c["kv"])
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        kept = len(paged._workspaces)
+        for keys in ([1, 2], None, torch.zeros(0, dtype=torch.bfloat16, device=DEV), wide[..., :0]):
+            with pytest.raises(ValueError):
+                paged.chunk_attention(out, c["q"], keys, keys, *rest, scale=0.1)
+        rows = torch.empty(2, 4 * 96, dtype=torch.bfloat16, device=DEV)
+        with pytest.raises(rt.LcrError) as e:
+            paged.chunk_attention(rows, rows.clone(), wide, wide, *rest, scale=0.1)
+        assert e.value.status == 2 and len(paged._workspaces) == kept
