@@ -546,6 +546,14 @@ LCR_API int lcr_verify_drafts(int32_t* tokens, int32_t* accepted, const float* t
                               int64_t target_stride, const int32_t* target_starts, const int32_t* drafts,
                               const int32_t* draft_counts, const float* draft_probs, const float* uniforms,
                               int sequences, int max_drafts, int vocab, lcr_stream_t stream);
+/* The same, told how many rows target_probs has: a request whose rows are not
+ * among them (malformed target_starts) counts as idle. lcr_verify_drafts goes
+ * wherever target_starts points. */
+LCR_API int lcr_verify_drafts_bounded(int32_t* tokens, int32_t* accepted, const float* target_probs,
+                                      int64_t target_stride, int target_rows, const int32_t* target_starts,
+                                      const int32_t* drafts, const int32_t* draft_counts, const float* draft_probs,
+                                      const float* uniforms, int sequences, int max_drafts, int vocab,
+                                      lcr_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -305,21 +305,30 @@ extern "C" int lcr_token_probs(float* probs, int64_t probs_stride, const float* 
   return launch_cluster(kernel, rows * ctas, ctas, kProbsThreads, sizeof(float) * std::min(a.slice, kProbsSlice), cs(stream), a);
 }
 
-extern "C" int lcr_verify_drafts(int32_t* tokens, int32_t* accepted, const float* target_probs, int64_t target_stride,
-                                 const int32_t* target_starts, const int32_t* drafts, const int32_t* draft_counts,
-                                 const float* draft_probs, const float* uniforms, int sequences, int max_drafts,
-                                 int vocab, lcr_stream_t stream) {
+extern "C" int lcr_verify_drafts_bounded(int32_t* tokens, int32_t* accepted, const float* target_probs,
+                                         int64_t target_stride, int target_rows, const int32_t* target_starts,
+                                         const int32_t* drafts, const int32_t* draft_counts, const float* draft_probs,
+                                         const float* uniforms, int sequences, int max_drafts, int vocab,
+                                         lcr_stream_t stream) {
   if (sequences == 0) return LCR_OK;
   LCRB_REQUIRE(tokens && accepted && target_probs && target_starts && draft_counts && uniforms && sequences > 0 &&
-                   max_drafts >= 0 && vocab > 0 && (max_drafts == 0 || drafts),
+                   target_rows >= 0 && max_drafts >= 0 && vocab > 0 && (max_drafts == 0 || drafts),
                LCR_ERR_INVALID, "verify_drafts: null pointer or bad size");
   LCRB_REQUIRE(target_stride >= vocab, LCR_ERR_INVALID, "verify_drafts: row stride %lld of %d ids",
                static_cast<long long>(target_stride), vocab);
-  VerifyArgs a = {tokens,      accepted, target_probs, target_stride, target_starts, drafts, draft_counts,
-                  draft_probs, uniforms, sequences,    max_drafts,    vocab};
+  VerifyArgs a = {tokens,       accepted,    target_probs, target_stride, target_rows, target_starts, drafts,
+                  draft_counts, draft_probs, uniforms,     sequences,     max_drafts,  vocab};
   // CTAs for a request: as many as run at once (two on an SM) for all of them
   // (64 requests of 128256 ids: 41, 25, 19.5 and 23 us with 1, 2, 4 and 8).
   int ctas = 1;
   while (ctas < kVerifyMaxCtas && static_cast<long long>(sequences) * ctas * 2 <= 296) ctas *= 2;
   return launch_cluster(verify_drafts_kernel, sequences * ctas, ctas, kVerifyThreads, 0, cs(stream), a);
+}
+
+extern "C" int lcr_verify_drafts(int32_t* tokens, int32_t* accepted, const float* target_probs, int64_t target_stride,
+                                 const int32_t* target_starts, const int32_t* drafts, const int32_t* draft_counts,
+                                 const float* draft_probs, const float* uniforms, int sequences, int max_drafts,
+                                 int vocab, lcr_stream_t stream) {
+  return lcr_verify_drafts_bounded(tokens, accepted, target_probs, target_stride, INT32_MAX, target_starts, drafts,
+                                   draft_counts, draft_probs, uniforms, sequences, max_drafts, vocab, stream);
 }

@@ -22,7 +22,7 @@ decltype(&lcr_plan_step) plan_step_c = nullptr;
 decltype(&lcr_qk_norm_rope_kv) qk_norm_rope_kv_c = nullptr;
 decltype(&lcr_chunk_attention) chunk_attention_c = nullptr;
 decltype(&lcr_token_probs) token_probs_c = nullptr;
-decltype(&lcr_verify_drafts) verify_drafts_c = nullptr;
+decltype(&lcr_verify_drafts_bounded) verify_drafts_c = nullptr;
 
 // A Python error is set.
 struct Refused {};
@@ -239,8 +239,8 @@ int verify_drafts(PyObject* const* args, Py_ssize_t nargs) {
                                           "contiguous Float [requests, max_drafts, vocab]");
   float* u = c.dense<float>(7, "uniforms", at::kFloat, n * (most + 1), {most + 1}, "contiguous Float [requests, max_drafts + 1]");
   return verify_drafts_c(static_cast<int32_t*>(t.data_ptr()), c.ints(1, "accepted", n), static_cast<const float*>(p.data_ptr()),
-                         p.stride(0), c.ints(3, "target_starts", n + 1), c.ints(4, "drafts", 0), c.ints(5, "draft_counts", n),
-                         q, u, n, k, vocab, c.stream());
+                         p.stride(0), c.small(p.size(0)), c.ints(3, "target_starts", n + 1), c.ints(4, "drafts", 0),
+                         c.ints(5, "draft_counts", n), q, u, n, k, vocab, c.stream());
 }
 
 template <int (*F)(PyObject* const*, Py_ssize_t)>
@@ -269,7 +269,7 @@ PyObject* open_library(PyObject*, PyObject* path) {
   };
   if (!(bind(plan_step_c, "lcr_plan_step") && bind(qk_norm_rope_kv_c, "lcr_qk_norm_rope_kv") &&
         bind(chunk_attention_c, "lcr_chunk_attention") && bind(token_probs_c, "lcr_token_probs") &&
-        bind(verify_drafts_c, "lcr_verify_drafts"))) {
+        bind(verify_drafts_c, "lcr_verify_drafts_bounded"))) {
     PyErr_SetString(PyExc_RuntimeError, "the library lacks an operator");
     return nullptr;
   }

@@ -18,6 +18,7 @@ struct VerifyArgs {
   int32_t* accepted;
   const float* target;
   long long target_stride;
+  int target_rows;
   const int32_t* target_starts;
   const int32_t* drafts;
   const int32_t* counts;
@@ -169,7 +170,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_drafts_kernel(const 
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int b = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r0 = a.target_starts[b], r1 = a.target_starts[b + 1];
-  if (r1 <= r0) {  // the same for the whole cluster
+  if (r1 <= r0 || r0 < 0 || r1 > a.target_rows) {  // the same for the whole cluster
     if (rank == 0) verify_write(a, b, -1, -1);
     cluster.barrier_wait();
     return;

@@ -123,7 +123,8 @@ def token_probs(probs, logits, temperature=None, row_sequence=None) -> None:
 def verify_drafts(tokens, accepted, target_probs, target_starts, drafts, draft_counts, draft_probs, uniforms) -> None:
     """Keeps each request's drafts as far as the given uniforms allow and draws
     its next token (``lcr_verify_drafts``). ``draft_probs`` [requests,
-    max_drafts, vocab], or None for drafts that were certain."""
+    max_drafts, vocab], or None for drafts that were certain. A request whose
+    ``target_starts`` are not among ``target_probs``' rows counts as idle."""
     status = (_lib or _operators()).verify_drafts(tokens, accepted, target_probs, target_starts, drafts, draft_counts,
                                                   draft_probs, uniforms)
     if status:

@@ -172,6 +172,7 @@ _SIGS = {
     "lcr_chunk_attention_status": (_I, [_V, _V]),
     "lcr_token_probs": (_I, [_V, _L, _V, _L, _I, _I, _V, _I, _V, _V]),
     "lcr_verify_drafts": (_I, [_V, _V, _V, _L, _V, _V, _V, _V, _V, _I, _I, _I, _V]),
+    "lcr_verify_drafts_bounded": (_I, [_V, _V, _V, _L, _I, _V, _V, _V, _V, _V, _I, _I, _I, _V]),
 }
 
 _lib: Optional[ctypes.CDLL] = None

@@ -171,3 +171,23 @@ def test_chunk_attention_checks_before_it_keeps_a_workspace():
         with pytest.raises(rt.LcrError) as e:
             paged.chunk_attention(rows, rows.clone(), wide, wide, *rest, scale=0.1)
         assert e.value.status == 2 and len(paged._workspaces) == kept
+
+
+@pytest.mark.parametrize("n,k,vocab", [(4, 2, 40), (4, 2, 128256), (300, 1, 50)])
+def test_verify_drafts_rows_outside_the_target(n, k, vocab):
+    """A request whose rows are not all among the target's is idle; the others
+    are as without it."""
+    g = torch.Generator(device=DEV).manual_seed(vocab)
+    p = torch.softmax(torch.randn(n * (k + 1), vocab, generator=g, device=DEV), 1)
+    starts = np.arange(n + 1) * (k + 1)
+    drafts, counts = np.full((n, k), 3), np.full(n, k)
+    u = torch.rand(n, k + 1, generator=g, device=DEV)
+    want = run_verify(p, starts, drafts, counts, None, u)
+    for where, bad in [(n, n * (k + 1) + 1), (n, 2 ** 30), (n, 2 ** 31 - 1), (0, -1), (0, -2 ** 31)]:
+        at = starts.copy()
+        at[where] = bad  # the last request passes the target's end, or the first begins before it
+        got = run_verify(p, at, drafts, counts, None, u)
+        idle = max(0, where - 1)
+        others = np.arange(n) != idle
+        assert (got[0][idle] == -1).all() and got[1][idle] == 0
+        assert np.array_equal(got[0][others], want[0][others]) and np.array_equal(got[1][others], want[1][others])
