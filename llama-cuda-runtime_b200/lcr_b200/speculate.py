@@ -135,6 +135,8 @@ class Speculator:
         for i, r in enumerate(requests):
             if len(r.prompt) == 0:
                 raise ValueError(f"request {i} has an empty prompt")
+            if not all(0 <= t < self.model.geom.vocab_size for t in r.prompt):
+                raise ValueError(f"request {i} has tokens outside the vocabulary of {self.model.geom.vocab_size}")
             # (The last token needs no place in the cache.)
             longest, holds = len(r.prompt) + max(1, r.new_tokens) - 1, self.model.tables.shape[1] * self.model.page_size
             if longest > holds:

@@ -17,6 +17,7 @@ class Rows:
 
     def __init__(self, slots=2, max_seq=48, page_size=16):
         self.w = types.SimpleNamespace(device=torch.device("cpu"))
+        self.geom = types.SimpleNamespace(vocab_size=VOCAB)
         self.slots, self.page_size = slots, page_size
         self.tables = torch.zeros(slots, -(-max_seq // page_size), dtype=torch.int32)
         self.kv_lengths = torch.zeros(slots, dtype=torch.int32)
@@ -99,3 +100,12 @@ def test_a_prompt_may_be_an_array():
     r = sp.Request(numpy.arange(1, 6), 3)
     sp.Speculator(Rows()).run([r])
     assert r.generated == greedy([1, 2, 3, 4, 5], 3)
+
+
+@pytest.mark.parametrize("token", [-1, VOCAB, 2 ** 31 - 1])
+def test_a_prompt_outside_the_vocabulary_is_refused(token):
+    """The embedding's table has no row for it."""
+    model = Rows()
+    with pytest.raises(ValueError, match="request 1 .*vocabulary"):
+        sp.Speculator(model).run([sp.Request([1], 2), sp.Request([3, token, 4], 2)])
+    assert not model.steps
