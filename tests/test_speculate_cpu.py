@@ -8,7 +8,7 @@ torch = pytest.importorskip("torch")
 
 from lcr_b200 import paged, speculate as sp  # noqa: E402
 
-VOCAB = 31
+VOCAB = 61
 
 
 class Rows:
