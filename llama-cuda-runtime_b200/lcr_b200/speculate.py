@@ -193,6 +193,8 @@ class Speculator:
                 r.cached += new[b]
                 continue
             a = int(accepted[b])
+            if kept[b, a] < 0:
+                raise ArithmeticError(f"request {b} has nothing to draw from at {len(r.tokens) + a}: its logits are not finite")
             r.cached = len(r.tokens) + a
             r.tokens += [int(t) for t in kept[b, :a + 1]]
             r.drafted += counts[b]

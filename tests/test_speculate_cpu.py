@@ -55,6 +55,8 @@ def plain_operators(monkeypatch):
                 while accepted[b] < counts[b] and drafts[b, accepted[b]] == best[accepted[b]]:
                     accepted[b] += 1
                 tokens[b, :accepted[b] + 1] = best[:accepted[b] + 1]
+                if probs[starts[b + 1] - 1 - counts[b] + accepted[b]].isnan().all():
+                    tokens[b, accepted[b]] = -1
 
     monkeypatch.setattr(paged, "token_probs", lambda *a: None)
     monkeypatch.setattr(paged, "verify_drafts", verify)
@@ -109,3 +111,18 @@ def test_a_prompt_outside_the_vocabulary_is_refused(token):
     with pytest.raises(ValueError, match="request 1 .*vocabulary"):
         sp.Speculator(model).run([sp.Request([1], 2), sp.Request([3, token, 4], 2)])
     assert not model.steps
+
+
+def test_a_row_without_a_token_is_an_error():
+    """Logits of NaN leave nothing to draw from: a token of -1 is not gone on
+    from, and not handed out."""
+    class Broken(Rows):
+        def forward(self, *a):
+            logits = super().forward(*a)
+            return logits * float("nan") if len(self.steps) == 3 else logits
+
+    requests = [sp.Request([1, 2], 8), sp.Request([4], 8)]
+    with pytest.raises(ArithmeticError, match="request .*nothing to draw"):
+        sp.Speculator(Broken(), drafts=0).run(requests)
+    assert all(0 <= t < VOCAB for r in requests for t in r.tokens)
+    assert [len(r.generated) for r in requests] == [2, 2]
