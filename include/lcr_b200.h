@@ -458,7 +458,8 @@ LCR_API int lcr_batch_time_steps(lcr_batch* batch, int steps, float* ms);
  * and -1, so that a step captured in a graph for max_rows rows runs with
  * fewer; rows past it are cut off (row_starts[sequences] is then max_rows, and
  * the request that is cut must not go on to lcr_chunk_attention).
- * pool_pages * page_size must fit in 31 bits. */
+ * At least one request; pool_pages * page_size, max_pages * page_size and
+ * sequences * max_pages must fit in 31 bits. */
 LCR_API int lcr_plan_step(int32_t* block_tables, int max_pages, const int32_t* held, int32_t* held_out,
                           int32_t* free_pages, const int32_t* free_count, int32_t* free_count_out,
                           int pool_pages, const int32_t* cached, const int32_t* new_tokens,

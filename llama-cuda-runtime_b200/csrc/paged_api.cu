@@ -124,6 +124,7 @@ extern "C" int lcr_plan_step(int32_t* block_tables, int max_pages, const int32_t
   LCRB_REQUIRE(sequences <= LCR_PLAN_MAX_SEQUENCES, LCR_ERR_SHAPE, "plan_step: %d requests; at most %d", sequences,
                LCR_PLAN_MAX_SEQUENCES);
   LCRB_REQUIRE(static_cast<long long>(sequences) * max_pages <= INT32_MAX &&
+                   static_cast<long long>(max_pages) * page_size <= INT32_MAX &&
                    static_cast<long long>(pool_pages) * page_size <= INT32_MAX,
                LCR_ERR_SHAPE, "plan_step: tables or pool pass 31 bits");
   StepPlanArgs a = {};
