@@ -1,4 +1,5 @@
-"""What `make` builds: the library with or without torch."""
+"""What `make` builds: the library with or without torch, and the tensor
+operators again when Python or torch is another."""
 import os
 import stat
 import subprocess
@@ -28,3 +29,8 @@ def script(tmp_path, body):
 def test_a_make_without_torch_leaves_the_tensor_operators_out(tmp_path, body):
     out = planned(script(tmp_path, body), "-W", TENSORS)
     assert "tensors.cpp" not in out and "_tensors.so is left out" in out
+
+
+def test_a_make_with_another_torch_builds_the_tensor_operators_again(tmp_path):
+    python = script(tmp_path, "echo py399-torch99.0\n")
+    assert "tensors.cpp" in planned(python)
