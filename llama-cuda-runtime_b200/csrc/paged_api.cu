@@ -321,8 +321,9 @@ extern "C" int lcr_verify_drafts_bounded(int32_t* tokens, int32_t* accepted, con
                   draft_counts, draft_probs, uniforms,     sequences,     max_drafts,  vocab};
   // CTAs for a request: as many as run at once (two on an SM) for all of them
   // (64 requests of 128256 ids: 41, 25, 19.5 and 23 us with 1, 2, 4 and 8).
+  const int sms = multiprocessors();
   int ctas = 1;
-  while (ctas < kVerifyMaxCtas && static_cast<long long>(sequences) * ctas * 2 <= 296) ctas *= 2;
+  while (ctas < kVerifyMaxCtas && static_cast<long long>(sequences) * ctas <= sms) ctas *= 2;
   return launch_cluster(verify_drafts_kernel, sequences * ctas, ctas, kVerifyThreads, 0, cs(stream), a);
 }
 
