@@ -156,6 +156,17 @@ def test_plan_step_from_several_threads():
     assert bad == {n: 0 for n in sizes}
 
 
+def test_chunk_attention_scratch_serves_both_head_sizes():
+    """Every call leaves a workspace ready for the next, whatever its head
+    size: tiles split over the whole GPU, in turn, on one workspace."""
+    a = attention_case([(5, 9000), (64, 3000)], 8, 2, 64, 16, seed=4)
+    b = attention_case([(3, 12000), (40, 2500)], 4, 1, 128, 16, seed=5)
+    space = max((paged.attention_workspace(8, d) for d in (64, 128)), key=torch.Tensor.numel)
+    for _ in range(2):
+        check_attention(b, run_attention(b, space))
+        check_attention(a, run_attention(a, space))
+
+
 def test_chunk_attention_checks_before_it_keeps_a_workspace():
     c = attention_case([(2, 20)], 4, 2, 64, 16)
     wide = torch.zeros(2, 2, 16, 96, dtype=torch.bfloat16, device=DEV)
@@ -191,3 +202,70 @@ def test_verify_drafts_rows_outside_the_target(n, k, vocab):
         others = np.arange(n) != idle
         assert (got[0][idle] == -1).all() and got[1][idle] == 0
         assert np.array_equal(got[0][others], want[0][others]) and np.array_equal(got[1][others], want[1][others])
+
+
+def counting_case(lens, heads, kv_heads, d, ps, *, left_out=None):
+    """Queries of zeros weigh all visible keys alike (1 each, exact), and key j
+    has a one in dimension j // width: a dimension of the result is the share
+    of the visible keys that fall to it. Returns the case and the 64-bit
+    result, without the keys `left_out` of each request."""
+    c = attention_case(lens, heads, kv_heads, d, ps)
+    c["q"].zero_()
+    want = torch.zeros(c["q"].shape[0], d, dtype=torch.float64, device=DEV)
+    for b, (n, kv) in enumerate(lens):
+        width = -(-kv // d)
+        j = torch.arange(kv, device=DEV)
+        page = torch.tensor(c["host_tables"][b].astype(np.int64), device=DEV)[j // ps]
+        v = torch.nn.functional.one_hot(j // width, d)
+        c["values"][page, :, j % ps] = v[:, None].bfloat16()
+        if left_out is not None:
+            v[left_out] = 0
+        sums = v.double().cumsum(0)[kv - n:]
+        r0 = int(c["host_starts"][b])
+        want[r0:r0 + n] = sums / sums.sum(1, keepdim=True)
+    return c, want[:, None].expand(-1, heads, -1).reshape(-1, heads * d)
+
+
+@pytest.mark.parametrize("lens,heads,kv_heads,d,ps", [
+    ([(1, 33000)], 1, 1, 64, 16), ([(1, 33000)], 1, 1, 128, 16), ([(1, 29001)], 1, 1, 64, 5),
+    ([(5, 30001)], 4, 1, 128, 16), ([(130, 20011)], 4, 1, 64, 16), ([(3, 9000), (1, 15000), (300, 4000)], 8, 2, 64, 16),
+    ([(2, 7000), (77, 5000)], 8, 2, 128, 16)])
+def test_chunk_attention_counts_every_key(lens, heads, kv_heads, d, ps):
+    """Sums of ones: the only roundings are those of 1 / l (2^-23), of the
+    product with it (2^-24) and to bf16 (2^-8), so a result is within 2^-7.9 of
+    the exact one (masked keys weigh 2^-125 at most); a block of keys left out,
+    planted in the reference, is far outside that."""
+    c, want = counting_case(lens, heads, kv_heads, d, ps)
+    near = lambda x: bool(((x.double() - want).abs() <= want * 2.0 ** -7.9 + 2.0 ** -115).all())  # noqa: E731
+    assert near(run_attention(c))
+    assert not near(counting_case(lens, heads, kv_heads, d, ps, left_out=slice(1024, 1088))[1])
+
+
+def one_request_reference(c, left_out=slice(0)):
+    """The 64-bit result of a case of one request, without the keys left out."""
+    (n, kv), d, group = c["lens"][0], c["d"], c["heads"] // c["kv_heads"]
+    page = torch.tensor(c["host_tables"][0].astype(np.int64), device=DEV)
+    k, v = (x[page].double().transpose(1, 2).reshape(-1, c["kv_heads"], d)[:kv] for x in (c["keys"], c["values"]))
+    seen = torch.arange(kv, device=DEV)[None] <= torch.arange(kv - n, kv, device=DEV)[:, None]
+    seen[:, left_out] = False
+    out = []
+    for h in range(c["heads"]):
+        s = c["q"][:, h * d:(h + 1) * d].double() @ k[:, h // group].T / math.sqrt(d)
+        out.append(torch.softmax(s.masked_fill(~seen, -math.inf), 1) @ v[:, h // group])
+    return torch.cat(out, 1)
+
+
+@pytest.mark.parametrize("lens,heads,kv_heads,d", [
+    ([(1, 33000)], 1, 1, 64), ([(5, 30001)], 4, 1, 128), ([(130, 20011)], 4, 1, 64)])
+def test_chunk_attention_rms_error(lens, heads, kv_heads, d):
+    """With random values the roundings are random too. To bf16 each is half a
+    unit in the last place at most, evenly spread: with leading digits m in
+    [1, 2) 2^-8 / (sqrt(3) m), 2^-9.2 rms. The weights' and the output's own
+    make 2^-8.7 of the result's rms together; 2^-8 is allowed. A bound on the largest error, which lets all roundings of a long
+    row point one way, would hide a lost range; 320 keys left out of the
+    reference show that this one does not."""
+    c = attention_case(lens, heads, kv_heads, d, 16, seed=31)
+    want = one_request_reference(c)
+    rms = lambda x: float(x.square().mean().sqrt())  # noqa: E731
+    assert rms(run_attention(c).double() - want) <= 2.0 ** -8 * rms(want)
+    assert rms(one_request_reference(c, slice(1024, 1344)) - want) > 2.0 ** -8 * rms(want)
