@@ -48,17 +48,19 @@
 // What it measured, with 32 query and 8 KV heads, and what bounds it:
 //   64 requests of 1 - 5 rows on 128 - 4096 keys, heads of 64: 59 us for 279 MB
 //     of keys and values, 4.7 TB/s, 0.72 of a copy's rate. Memory, and 9 us of
-//     start (the scan, the first loads) and of joining split tiles.
+//     start (the scan, the first loads) and of joining split tiles. (With one row
+//     each 58 us, and 100 with heads of 128, 5.6 TB/s.)
 //   15 of these beside a chunk of 509 rows, heads of 128: 42 us for 130 MB, 0.47
 //     of a copy's rate. The chain of a block, 4 - 5 thousand cycles while loads
 //     come late, about ten blocks a CTA.
-//   2048 rows on 32768 keys, heads of 64: 801 us (790 - 815 between runs), 665
-//     TFLOP/s, 0.39 of a large product's rate. The chain again: 2900 cycles a block, of them 1500 in the
-//     softmax warps (shared with the other CTAs'), the rest the way to the tensor
-//     cores and back; tensor cores 41 % and transcendental pipe 50 % busy, issue
-//     slots 57 %.
-//   2048 rows on 8192 keys, heads of 128: 266 us, 900 TFLOP/s. The keys and
-//     values that each tile of 128 pairs reads again, 6.7 TB/s out of L2.
+//   2048 rows on 32768 keys, heads of 64: 806 us (790 - 828 between runs), 661
+//     TFLOP/s, 0.39 of a large product's rate. The chain again: 2900 cycles a
+//     block, of them 1500 in the softmax warps (shared with the other CTAs'), the
+//     rest the way to the tensor cores and back; tensor cores 41 % and
+//     transcendental pipe 50 % busy, issue slots 57 %.
+//   2048 rows on 8192 keys, heads of 128: 275 us, 873 TFLOP/s, 0.52. The chain, two
+//     of them an SM, and a ring that holds one block's K and V: tensor cores 45 %,
+//     transcendental pipe 37 %, issue slots 39 %; 2 GB out of L2, which is 27 % busy.
 //   5 rows on 250 keys, heads of 64: 9.8 us, latency from end to end.
 // Measured and no faster: P signalled in halves, so that P V starts early (812
 // us for the third case, 811 without); the last 32 scores kept in registers
@@ -93,7 +95,9 @@ template <int BLK>
 constexpr int ca_min_range() {  // units of a range at least (where there are as many); at least ca_reach
   return ca_reach<BLK>();
 }
-// Of 8 pairs of exponentials, on the FMA pipe (2048 rows on 32768 keys: 801 us, with none 814).
+// Of 8 pairs of exponentials, on the FMA pipe (2048 rows on 32768 keys: 806 us, with
+// none 828, medians of 40 runs of each in turn; 59 and 43 us with either in the
+// first two cases).
 constexpr int kCaFmaGroups = 1;
 
 struct ChunkAttnArgs {

@@ -62,9 +62,9 @@ constexpr int kQkCtas = 4;   // per SM
 // loads the next row's pieces (64 bytes a thread), position and slot before it
 // works on the present one, so that loads are always in flight; the angles'
 // pairs, by head_dim / 2 threads, are double-buffered, with one barrier a row.
-// 8192 rows of 32 + 16 heads of 128: 36.7 us for 201 MB, 5.5 TB/s, 0.84 of a
-// copy's rate (a CTA for each row, without loads ahead: 51); 320 rows of heads
-// of 64: 2.5 us, latency.
+// 8192 rows of 32 + 16 heads of 128: 37.0 us for 201 MB, 5.4 TB/s, 0.83 of a
+// copy's rate, and 34.1 us without norms (a CTA for each row, without loads
+// ahead: 51); 320 rows of heads of 64: 2.7 us, latency.
 template <int D>
 __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kernel(const QkNormRopeArgs a) {
   constexpr int HALF = D / 2;

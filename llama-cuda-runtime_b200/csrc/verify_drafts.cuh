@@ -158,8 +158,9 @@ __device__ __forceinline__ void verify_write(const VerifyArgs& a, int b, int kep
 //
 // A chain of latencies (the draft, its two probabilities, the row, the exchange,
 // the chunk) around the row's reading: one request of four drafts over 128256
-// ids 8.5 us; 64 of them, 49 MB, 19.5 us, 2.5 TB/s (with conversions to 64 bits
-// in place of verify_split, 41; with each half chunk loaded ahead, 21).
+// ids 8.6 us; 64 of them, 49 MB, 19.8 us, 2.5 TB/s (with conversions to 64 bits
+// in place of verify_split, 41; with each half chunk loaded ahead, 21). With
+// certain drafts 7.4 and 15.3 us.
 __global__ void __launch_bounds__(kVerifyThreads, 2) verify_drafts_kernel(const VerifyArgs a) {
   __shared__ int kept_s;
   __shared__ long long sums[kVerifyChunks];
